@@ -13,9 +13,10 @@ import os
 
 import torch
 
-from afd_plugin_b200.ops import checks
+from afd_plugin_b200.ops import checks, kv_int4
 from afd_plugin_b200.ops import reference as ref
 from afd_plugin_b200.ops._ext import ops as _cuda_ops
+from afd_plugin_b200.ops.kv_int4 import Int4KV, int4_kv_cache
 
 SCORING_IDS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 
@@ -323,6 +324,72 @@ def gqa_prologue(
     return q
 
 
+# ----------------------------------------------------------- 4-bit KV cache
+def gqa_cache_write_int4(
+    kv: Int4KV, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, scores: torch.Tensor | None = None
+) -> None:
+    """Quantise ``k`` / ``v [T, kv_heads, d]`` (bf16, fp16 or fp32; last dim dense) into the cache slots.
+
+    The slots of one call should differ (rows written to one slot leave a mix of them; padding rows
+    share the padding block that way).  A slot outside the cache is skipped and sets the device
+    status word.  ``scores`` (the cache's accumulated attention weights) restart at zero there.
+    Values must be finite for their 64-dim group to keep a meaning.
+    """
+    if checks.enabled():
+        checks.cache_slots("gqa_cache_write_int4", slot_mapping, num_slots=kv.num_blocks * kv.block_size)
+    if _cuda(k):
+        _cuda_ops().gqa_cache_write_int4(*kv, k, v, slot_mapping, scores)
+        return
+    kv_int4.check_cache("gqa_cache_write_int4", kv, scores)
+    kv_int4.check_rows("gqa_cache_write_int4", kv, k, v, slot_mapping)
+    ref.gqa_cache_write_int4(kv, k, v, slot_mapping, scores)
+
+
+def gqa_cache_read_int4(
+    kv: Int4KV, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values stored at ``slots [n]`` (int64): ``(k, v)``, each ``[n, kv_heads, d]`` in ``dtype``."""
+    if checks.enabled():
+        checks.cache_slots("gqa_cache_read_int4", slots, num_slots=kv.num_blocks * kv.block_size)
+    if _cuda(slots):
+        return _cuda_ops().gqa_cache_read_int4(*kv, slots, dtype)
+    kv_int4.check_cache("gqa_cache_read_int4", kv)
+    kv_int4.check_slots("gqa_cache_read_int4", slots)
+    return ref.gqa_cache_read_int4(kv, slots, dtype)
+
+
+def gqa_decode_int4(
+    q: torch.Tensor,
+    kv: Int4KV,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float,
+    *,
+    scores: torch.Tensor | None = None,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Single-token attention ``[B, heads, d]`` of ``q [B, heads, d]`` (bf16 / fp16) over the 4-bit cache.
+
+    An empty sequence gives zeros (and a log-sum-exp of ``-inf``).  With ``return_lse`` also the
+    natural log-sum-exp of every row, fp32 ``[B, heads]``.  With ``scores``
+    (``[blocks, kv_heads, block_size]`` fp32) each cached position's attention weight, summed over
+    the query heads that share its KV head, is added to its entry: the weight :func:`kv_evict_int4`
+    keeps positions by.  Sequences of a batch that share blocks add to the same entries, in no fixed
+    order.
+    """
+    if checks.enabled():
+        checks.paged_attention("gqa_decode_int4", block_table, seq_lens, num_blocks=kv.num_blocks,
+                               block_size=kv.block_size, min_len=0)
+    if _cuda(q):
+        out, lse = _cuda_ops().gqa_decode_int4(q, *kv, block_table, seq_lens, scale, scores, return_lse)
+    else:
+        kv_int4.check_cache("gqa_decode_int4", kv, scores)
+        kv_int4.check_query("gqa_decode_int4", kv, q)
+        kv_int4.check_batch("gqa_decode_int4", block_table, seq_lens, q.shape[0])
+        out, lse = ref.gqa_decode_int4(q, kv, block_table, seq_lens, scale, scores)
+    return (out, lse) if return_lse else out
+
+
 # -------------------------------------------------------------------- MoE
 def moe_experts(
     x: torch.Tensor,
@@ -410,12 +477,17 @@ def argmax(logits: torch.Tensor) -> torch.Tensor:
 
 
 __all__ = [
+    "Int4KV",
     "argmax",
     "dense_mlp",
     "fused_add_rms_norm",
+    "gqa_cache_read_int4",
     "gqa_cache_write",
+    "gqa_cache_write_int4",
     "gqa_decode",
+    "gqa_decode_int4",
     "head_linear",
+    "int4_kv_cache",
     "linear",
     "mla_cache_write",
     "mla_decode",

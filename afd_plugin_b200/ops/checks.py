@@ -45,17 +45,17 @@ def _first_bad(mask: torch.Tensor) -> tuple[int, ...] | None:
 
 
 def paged_attention(op: str, block_table: torch.Tensor, seq_lens: torch.Tensor, *, num_blocks: int,
-                    block_size: int) -> None:
-    """Every block a sequence reaches is a real block; lengths fit the table."""
+                    block_size: int, min_len: int = 1) -> None:
+    """Every block a sequence reaches is a real block; lengths fit the table (``min_len`` 0: may be empty)."""
     if not _active(block_table):
         return
     bt = block_table.detach().to("cpu", torch.int64)
     sl = seq_lens.detach().to("cpu", torch.int64).view(-1)
     if bt.dim() != 2 or bt.shape[0] < sl.shape[0]:
         raise KernelInputError(f"{op}: block table {tuple(bt.shape)} has fewer rows than {sl.shape[0]} sequences")
-    bad = _first_bad((sl < 1) | (sl > bt.shape[1] * block_size))
+    bad = _first_bad((sl < min_len) | (sl > bt.shape[1] * block_size))
     if bad is not None:
-        raise KernelInputError(f"{op}: seq_lens[{bad[0]}] = {int(sl[bad[0]])} outside [1, "
+        raise KernelInputError(f"{op}: seq_lens[{bad[0]}] = {int(sl[bad[0]])} outside [{min_len}, "
                                f"{bt.shape[1] * block_size}] (table width {bt.shape[1]} x block {block_size})")
     used = torch.arange(bt.shape[1])[None, :] < ((sl + block_size - 1) // block_size)[:, None]
     rows = bt[: sl.shape[0]]

@@ -1,13 +1,17 @@
 // torch.ops.afd_b200.* registrations for the sm_100a kernels.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdlib>
+#include <limits>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "launchers.h"
@@ -443,6 +447,224 @@ at::Tensor gqa_decode(const at::Tensor& q, const at::Tensor& kc, const at::Tenso
                     splits > 1 ? pl.data_ptr<float>() : nullptr, status_ptr(q), B, hq, hkv, 128, bs, nblocks,
                     (int)block_table.stride(0), splits, (float)scale, stream());
   return out;
+}
+
+// ------------------------------------------------------- 4-bit KV cache
+// The status word, or null where it would first have to be made inside a graph capture.
+int* status_ptr_or_null(const at::Tensor& like) {
+  const int device = like.get_device();
+  {
+    std::lock_guard<std::mutex> lock(g_status_mu);
+    if ((int)g_status.size() > device && g_status[device].defined()) return g_status[device].data_ptr<int>();
+  }
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
+  return status_ptr(like);
+}
+
+// Numbers in messages go through std::to_string: the extension may carry its own
+// copy of the C++ runtime, whose stream formatting of numbers is not usable here.
+struct Kv4Shape {
+  int blocks, kv_heads, block_size, dim;
+};
+
+void check_same_device(const at::Tensor& t, const at::Tensor& like, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), op, ": ", name, " must be on cuda:",
+              std::to_string(like.get_device()));
+}
+
+Kv4Shape check_kv4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs,
+                   const char* op) {
+  TORCH_CHECK(kc.dim() == 4 && ks.dim() == 5, op, ": codes [blocks, kv_heads, block_size, dim / 2], scales "
+              "[blocks, kv_heads, block_size, dim / 64, 2]");
+  const int64_t d = kc.size(3) * 2;
+  TORCH_CHECK(d == 64 || d == 128 || d == 256, op, ": head dim 64, 128 or 256, got ", std::to_string(d));
+  TORCH_CHECK(kc.size(2) > 0 && kc.size(2) % 16 == 0, op, ": block size must be a multiple of 16, got ",
+              std::to_string(kc.size(2)));
+  TORCH_CHECK(kc.size(0) > 0 && kc.size(1) > 0 && kc.size(0) <= INT32_MAX && kc.size(1) <= 65535 &&
+                  kc.size(2) <= INT32_MAX / 2, op, ": empty or oversized cache");
+  for (const at::Tensor* t : {&kc, &vc}) {
+    TORCH_CHECK(t->scalar_type() == at::kByte && t->sizes() == kc.sizes(), op, ": uint8 codes of one shape");
+  }
+  for (const at::Tensor* t : {&ks, &vs}) {
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 5 && t->size(0) == kc.size(0) &&
+                    t->size(1) == kc.size(1) && t->size(2) == kc.size(2) && t->size(3) == d / 64 && t->size(4) == 2,
+                op, ": bf16 (step, zero) pairs per position and 64 dims");
+  }
+  for (const at::Tensor* t : {&kc, &ks, &vc, &vs}) {
+    check_same_device(*t, kc, op, "the cache");
+    TORCH_CHECK(t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, op,
+                ": contiguous, 16-byte aligned cache tensors");
+  }
+  return {(int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)d};
+}
+
+float* check_kv4_scores(const c10::optional<at::Tensor>& scores, const at::Tensor& kc, const char* op) {
+  if (!scores.has_value()) return nullptr;
+  check_same_device(*scores, kc, op, "scores");
+  TORCH_CHECK(scores->scalar_type() == at::kFloat && scores->is_contiguous() && scores->dim() == 3 &&
+                  scores->size(0) == kc.size(0) && scores->size(1) == kc.size(1) && scores->size(2) == kc.size(2),
+              op, ": fp32 contiguous scores [blocks, kv_heads, block_size]");
+  return scores->data_ptr<float>();
+}
+
+void check_kv4_batch(const at::Tensor& table, const at::Tensor& lens, const at::Tensor& kc, int64_t batch,
+                     const char* op) {
+  check_same_device(table, kc, op, "block_table");
+  check_same_device(lens, kc, op, "seq_lens");
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == batch &&
+                  (table.size(1) <= 1 || table.stride(1) == 1), op, ": int32 block_table [batch, blocks], dense rows");
+  TORCH_CHECK(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == batch &&
+                  (batch <= 1 || lens.stride(0) == 1), op, ": int32 seq_lens [batch]");
+  TORCH_CHECK(table.size(1) * kc.size(2) <= INT32_MAX, op, ": a table row covers at most 2^31 - 1 positions");
+}
+
+void gqa_cache_write_int4(at::Tensor& kc, at::Tensor& ks, at::Tensor& vc, at::Tensor& vs, const at::Tensor& k,
+                          const at::Tensor& v, const at::Tensor& slots, const c10::optional<at::Tensor>& scores) {
+  const char* op = "gqa_cache_write_int4";
+  check_cuda(kc, "the cache");
+  const Kv4Shape sh = check_kv4(kc, ks, vc, vs, op);
+  for (const at::Tensor* t : {&k, &v}) {
+    check_same_device(*t, kc, op, "k / v");
+    TORCH_CHECK(t->dim() == 3 && t->size(1) == sh.kv_heads && t->size(2) == sh.dim && t->stride(2) == 1 &&
+                    t->size(0) == k.size(0) && t->scalar_type() == k.scalar_type(),
+                op, ": k / v [tokens, kv_heads, dim] of one type, dense rows");
+  }
+  const int dt = dtype_code(k);
+  check_same_device(slots, kc, op, "slot_mapping");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                  slots.size(0) == k.size(0), op, ": int64 slot_mapping [tokens]");
+  TORCH_CHECK(k.size(0) <= INT32_MAX, op, ": at most 2^31 - 1 tokens");
+  Kv4WriteParams p{};
+  p.scores = check_kv4_scores(scores, kc, op);
+  if (k.size(0) == 0) return;
+  c10::cuda::CUDAGuard g(kc.device());
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_st = k.stride(0);
+  p.k_sh = k.stride(1);
+  p.v_st = v.stride(0);
+  p.v_sh = v.stride(1);
+  const int64_t per16 = 16 / k.element_size();
+  p.vec = 1;
+  for (const at::Tensor* t : {&k, &v})
+    if (reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0 || t->stride(0) % per16 != 0 || t->stride(1) % per16 != 0)
+      p.vec = 0;
+  p.slots = slots.data_ptr<int64_t>();
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.v_codes = vc.data_ptr<uint8_t>();
+  p.k_scale = reinterpret_cast<uint32_t*>(ks.data_ptr());
+  p.v_scale = reinterpret_cast<uint32_t*>(vs.data_ptr());
+  p.status = status_ptr_or_null(kc);
+  p.num_slots = (int64_t)sh.blocks * sh.block_size;
+  p.tokens = (int)k.size(0);
+  p.kv_heads = sh.kv_heads;
+  p.dim = sh.dim;
+  p.block_size = sh.block_size;
+  launch_kv4_write(p, dt, stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+std::tuple<at::Tensor, at::Tensor> gqa_cache_read_int4(const at::Tensor& kc, const at::Tensor& ks,
+                                                       const at::Tensor& vc, const at::Tensor& vs,
+                                                       const at::Tensor& slots, at::ScalarType dtype) {
+  const char* op = "gqa_cache_read_int4";
+  check_cuda(kc, "the cache");
+  const Kv4Shape sh = check_kv4(kc, ks, vc, vs, op);
+  check_same_device(slots, kc, op, "slots");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                  slots.size(0) <= INT32_MAX, op, ": int64 slots [tokens]");
+  c10::cuda::CUDAGuard g(kc.device());
+  const int64_t n = slots.size(0);
+  auto k = at::empty({n, sh.kv_heads, sh.dim}, kc.options().dtype(dtype));
+  auto v = at::empty_like(k);
+  const int dt = dtype_code(k);
+  if (n == 0) return {k, v};
+  Kv4ReadParams p{};
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.slots = slots.data_ptr<int64_t>();
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.v_codes = vc.data_ptr<uint8_t>();
+  p.k_scale = reinterpret_cast<const uint32_t*>(ks.data_ptr());
+  p.v_scale = reinterpret_cast<const uint32_t*>(vs.data_ptr());
+  p.status = status_ptr_or_null(kc);
+  p.num_slots = (int64_t)sh.blocks * sh.block_size;
+  p.tokens = (int)n;
+  p.kv_heads = sh.kv_heads;
+  p.dim = sh.dim;
+  p.block_size = sh.block_size;
+  launch_kv4_read(p, dt, stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> gqa_decode_int4(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& ks,
+                                                   const at::Tensor& vc, const at::Tensor& vs,
+                                                   const at::Tensor& table, const at::Tensor& lens, double scale,
+                                                   const c10::optional<at::Tensor>& scores, bool want_lse) {
+  const char* op = "gqa_decode_int4";
+  check_cuda(kc, "the cache");
+  const Kv4Shape sh = check_kv4(kc, ks, vc, vs, op);
+  check_same_device(q, kc, op, "q");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, op, ": q must be bf16 or fp16");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == sh.dim && q.stride(2) == 1, op, ": q [batch, heads, dim], dense rows");
+  const int64_t B = q.size(0), heads = q.size(1);
+  TORCH_CHECK(heads > 0 && heads % sh.kv_heads == 0 && heads <= 65535, op, ": heads must be a multiple of kv_heads");
+  check_kv4_batch(table, lens, kc, B, op);
+  float* sc = check_kv4_scores(scores, kc, op);
+  c10::cuda::CUDAGuard g(kc.device());
+  auto out = at::empty({B, heads, sh.dim}, q.options());
+  const bool lse_on = want_lse || sc != nullptr;
+  auto lse = at::empty({lse_on ? B : 0, heads}, q.options().dtype(at::kFloat));
+  if (B == 0) return {out, lse};
+  if (table.size(1) == 0) {  // no position anywhere
+    out.zero_();
+    lse.fill_(-std::numeric_limits<float>::infinity());
+    return {out, lse};
+  }
+  Kv4DecodeParams p{};
+  p.q_sb = q.stride(0);
+  p.q_sh = q.stride(1);
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.v_codes = vc.data_ptr<uint8_t>();
+  p.k_scale = reinterpret_cast<const uint32_t*>(ks.data_ptr());
+  p.v_scale = reinterpret_cast<const uint32_t*>(vs.data_ptr());
+  p.scores = sc;
+  p.table_stride = table.stride(0);
+  p.status = status_ptr_or_null(kc);
+  p.heads = (int)heads;
+  p.kv_heads = sh.kv_heads;
+  p.dim = sh.dim;
+  p.block_size = sh.block_size;
+  p.num_blocks = sh.blocks;
+  p.max_blocks = (int)table.size(1);
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  const int max_len = p.max_blocks * p.block_size;
+  for (int64_t b0 = 0; b0 < B;) {
+    const Kv4Plan plan = kv4_decode_plan((int)std::min<int64_t>(B - b0, 1 << 20), p.heads, p.kv_heads, p.dim, max_len);
+    const int64_t n = std::min<int64_t>(B - b0, plan.max_batch);
+    const Kv4Plan here = kv4_decode_plan((int)n, p.heads, p.kv_heads, p.dim, max_len);
+    p.batch = (int)n;
+    p.head_tiles = here.head_tiles;
+    p.chunks = here.chunks;
+    p.ctas = here.ctas;
+    p.direct = here.direct;
+    at::Tensor po, pm;
+    if (!here.direct) {
+      po = at::empty({2 * here.ctas, 8 * here.head_tiles, sh.dim}, q.options().dtype(at::kFloat));
+      pm = at::empty({2 * here.ctas, 8 * here.head_tiles, 2}, q.options().dtype(at::kFloat));
+      p.part_o = po.data_ptr<float>();
+      p.part_ml = pm.data_ptr<float>();
+    }
+    p.q = static_cast<const char*>(q.data_ptr()) + b0 * q.stride(0) * q.element_size();
+    p.out = static_cast<char*>(out.data_ptr()) + b0 * heads * sh.dim * out.element_size();
+    p.lse = lse_on ? lse.data_ptr<float>() + b0 * heads : nullptr;
+    p.block_table = table.data_ptr<int32_t>() + b0 * table.stride(0);
+    p.seq_lens = lens.data_ptr<int32_t>() + b0;
+    C10_CUDA_CHECK((cudaError_t)launch_gqa_decode_int4(p, dtype_code(q), stream()));
+    b0 += n;
+  }
+  return {out, lse};
 }
 
 // -------------------------------------------------------------------- MoE
@@ -1161,6 +1383,12 @@ TORCH_LIBRARY(afd_b200, m) {
         "int num_splits) -> Tensor");
   m.def("gqa_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, float scale, "
         "int num_splits) -> Tensor");
+  m.def("gqa_cache_write_int4(Tensor(a!) kc, Tensor(b!) ks, Tensor(c!) vc, Tensor(d!) vs, Tensor k, Tensor v, "
+        "Tensor slots, Tensor(e!)? scores) -> ()");
+  m.def("gqa_cache_read_int4(Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor slots, ScalarType dtype) -> "
+        "(Tensor, Tensor)");
+  m.def("gqa_decode_int4(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor block_table, Tensor seq_lens, "
+        "float scale, Tensor(a!)? scores, bool return_lse) -> (Tensor, Tensor)");
   m.def("moe_align(Tensor topk_ids, int e_local, int offset, int n_shared) -> Tensor[]");
   m.def("moe_gather(Tensor x, Tensor row_token, Tensor total) -> Tensor");
   m.def("grouped_gemm(Tensor a, Tensor w, Tensor offsets, Tensor counts, int epilogue) -> Tensor");
@@ -1220,6 +1448,9 @@ TORCH_LIBRARY_IMPL(afd_b200, CUDA, m) {
   m.impl("mla_decode", &mla_decode);
   m.impl("mla_decode_sparse", &mla_decode_sparse);
   m.impl("gqa_decode", &gqa_decode);
+  m.impl("gqa_cache_write_int4", &gqa_cache_write_int4);
+  m.impl("gqa_cache_read_int4", &gqa_cache_read_int4);
+  m.impl("gqa_decode_int4", &gqa_decode_int4);
   m.impl("moe_align", &moe_align);
   m.impl("moe_gather", &moe_gather);
   m.impl("grouped_gemm", &grouped_gemm);

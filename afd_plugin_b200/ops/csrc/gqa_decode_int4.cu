@@ -1,0 +1,805 @@
+// Grouped-query paged decode over the 4-bit KV cache (layout: kv_int4.cuh).
+//
+//   s[h, t] = scale * q_h . k_t        k_t = zk_t + ck_t * stepk_t   per 64 dims
+//   o_h     = sum_t softmax_t(s[h, :]) v_t
+//
+// With codes shifted to c - 8 (and zero to zero + 8 step) the products split:
+//   q . k_t = sum_groups step_t,j * (q_j . c_t,j) + zero_t,j * sum(q_j)
+//   o       = sum_groups (p_t step_t,j) c_t,j + p_t zero_t,j
+// so the tensor cores multiply q (exact in its own type) and p * step with
+// small integers (exact in bf16 / fp16), and the scales stay outside in fp32.
+// p * step is rounded to bf16 for the second product (8 bits: fp16 would not
+// hold the range of the steps); everything else, the running maximum and sum
+// included, is fp32.
+//
+// What bounds it: the packed rows, 144 B per position and KV head at D = 128,
+// at the HBM rate.  A warp unpacks the codes it needs straight into MMA
+// operand registers, so the tile is the A operand (16 positions x 16 dims, or
+// 16 dims x 16 positions) and the query heads are the 8 columns of B: a group
+// of 8 query heads needs half the MMAs that padding the heads to 16 rows
+// would.  Each warp owns whole 16-position tiles: a private ring of cp.async
+// stages, no block barrier in the loop, running maximum and sum per warp; the
+// warps of a CTA merge once at the end.
+//
+// Work split: a tile is 16 positions of one (sequence, KV head).  All tiles of
+// the batch, in (sequence, head, position) order, are dealt to one wave of
+// CTAs in equal contiguous shares, whatever the lengths; a share that covers
+// part of a (sequence, head) leaves a partial (unnormalised o, max, sum) that
+// a second small kernel joins.  Short tables (at most kDirectTiles tiles per
+// sequence) take one CTA per (sequence, head) instead and write the result at
+// once: one launch.
+//
+// Scores: a second pass over K alone, with the joined log-sum-exp, adds each
+// position's probability (summed over the group's query heads) to its score.
+#include "device_state.h"
+#include "kv_int4.cuh"
+#include "launchers.h"
+
+namespace afd {
+namespace kv4 {
+
+constexpr int kTile = 16;
+constexpr int kWarps = 8;
+constexpr int kDecThreads = kWarps * 32;
+constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
+constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
+
+template <int D>
+struct Ring {
+  static constexpr int kCodes = kTile * D / 2;          // bytes of one tile's codes
+  static constexpr int kPairs = kTile * (D / kGroup) * 4;
+  static constexpr int kHalf = kCodes + kPairs;  // K codes, K pairs; then the same of V
+  static constexpr int kStageBytes = 2 * kHalf;
+};
+
+// 16-byte chunk of a row of codes -> chunk in shared memory.  The MMA operand
+// loads of one instruction touch rows {0, 1, 2, 3}, {4, .., 7} (V) or
+// {0, 4, 1, 5}, {2, 6, 3, 7} (K); this spreads each set over all banks.
+template <int D>
+AFD_DEVICE int swz(int row, int chunk) {
+  if constexpr (D == 256) return chunk ^ (((row & 3) ^ ((row >> 1) & 2)) << 1);
+  if constexpr (D == 128) return chunk ^ ((((row >> 1) ^ (row >> 2)) & 1) << 1);
+  return chunk;
+}
+
+template <typename T> struct Codes;  // nibble pairs -> two values c - 8 of T
+template <> struct Codes<__nv_bfloat16> {
+  // 0x4300 | c is 128 + c in bf16; minus 136 is exact.
+  static AFD_DEVICE uint32_t pair(uint32_t w) {
+    const uint32_t m = (w & 0x000F000Fu) | 0x43004300u;
+    __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), __floats2bfloat162_rn(136.f, 136.f));
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+template <> struct Codes<__half> {
+  // 0x6400 | c is 1024 + c in fp16; minus 1032 is exact.
+  static AFD_DEVICE uint32_t pair(uint32_t w) {
+    const uint32_t m = (w & 0x000F000Fu) | 0x64006400u;
+    __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+
+template <typename T> AFD_DEVICE void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1);
+template <> AFD_DEVICE void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <> AFD_DEVICE void mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8x8 transpose of 16-bit values held one row pair per lane.
+AFD_DEVICE uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+AFD_DEVICE float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+AFD_DEVICE void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+AFD_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> AFD_DEVICE void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+AFD_DEVICE void lds64(uint32_t& a, uint32_t& b, uint32_t addr) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
+}
+AFD_DEVICE uint32_t lds32(uint32_t addr) {
+  uint32_t a;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a) : "r"(addr));
+  return a;
+}
+
+// Sequence length as the kernels use it: never negative, never past the table.
+AFD_DEVICE int seq_len_of(const Kv4DecodeParams& p, int b) {
+  const int n = p.seq_lens[b];
+  return n < 0 ? 0 : min(n, p.max_blocks * p.block_size);
+}
+
+// Row of a tile that MMA row (or k index) i stands for: rows are taken in the
+// order 0 4 1 5 2 6 3 7 (+ 8), which keeps both operands' loads conflict-free.
+AFD_DEVICE int tile_row(int i) { return (i & 8) | ((i & 7) >> 1) | ((i & 1) << 2); }
+
+// Inclusive prefix sums of the sequences' tile counts into cum[1 .. batch]
+// (cum[0] = 0); every thread of the block calls this.
+AFD_DEVICE void tile_prefix(const Kv4DecodeParams& p, int* cum, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, nw = blockDim.x / 32;
+  int carry = 0;
+  if (threadIdx.x == 0) cum[0] = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += blockDim.x) {
+    const int b = b0 + threadIdx.x;
+    int v = b < p.batch ? (seq_len_of(p, b) + kTile - 1) / kTile : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) warp_sums[warp] = v;
+    __syncthreads();
+    int before = carry, total = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += warp_sums[w];
+      total += warp_sums[w];
+    }
+    if (b < p.batch) cum[b + 1] = before + v;
+    carry += total;
+    __syncthreads();
+  }
+  __syncthreads();
+}
+
+// The share of tiles a CTA takes (the same expression wherever it is needed).
+AFD_DEVICE int64_t tiles_per_cta(int64_t total, int ctas) { return (total + ctas - 1) / ctas; }
+
+// One piece: tiles [t0, t1) of (sequence b, head chunk hv).
+struct Piece {
+  int b, hv, t0, t1;
+  bool whole;  // covers all tiles of (b, hv)
+};
+
+// Finds the piece that starts at position `at` of the batch's tile order and
+// ends at `end` or at its (sequence, head)'s last tile.
+AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, int64_t end) {
+  int lo = 0, hi = batch - 1;  // largest b with cum[b] * heads_v <= at
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int64_t)cum[mid] * heads_v <= at) lo = mid;
+    else hi = mid - 1;
+  }
+  const int tiles = cum[lo + 1] - cum[lo];
+  const int64_t rem = at - (int64_t)cum[lo] * heads_v;
+  Piece pc;
+  pc.b = lo;
+  pc.hv = (int)(rem / tiles);
+  pc.t0 = (int)(rem % tiles);
+  pc.t1 = (int)min((int64_t)tiles, pc.t0 + (end - at));
+  pc.whole = pc.t0 == 0 && pc.t1 == tiles;
+  return pc;
+}
+
+// A warp's view of one (sequence, KV head) in the cache.
+template <int D>
+struct TileSource {
+  const uint8_t *kc, *vc;
+  const uint8_t *ks, *vs;  // (step, zero) pairs, bytes
+  const int32_t* table;
+  int64_t head_off;        // first position of the head inside a block's rows
+  int64_t block_rows;      // rows (head, position) of one block
+  int block_size, num_blocks;
+  int* status;
+
+  AFD_DEVICE TileSource(const Kv4DecodeParams& p, int b, int kv_head)
+      : kc(p.k_codes), vc(p.v_codes), ks(reinterpret_cast<const uint8_t*>(p.k_scale)),
+        vs(reinterpret_cast<const uint8_t*>(p.v_scale)), table(p.block_table + (int64_t)b * p.table_stride),
+        head_off((int64_t)kv_head * p.block_size), block_rows((int64_t)p.kv_heads * p.block_size),
+        block_size(p.block_size), num_blocks(p.num_blocks), status(p.status) {}
+
+  // First cache row of tile t.  A block id outside the pool is reported and
+  // replaced by the padding block.
+  AFD_DEVICE int64_t row_of(int t) const {
+    const int pos = t * kTile;
+    const int pg = pos / block_size;
+    int blk = table[pg];
+    if ((unsigned)blk >= (unsigned)num_blocks) {
+      if (status != nullptr) atomicExch(status, kStatusBadIndex);
+      blk = 0;
+    }
+    return blk * block_rows + head_off + (pos - pg * block_size);
+  }
+
+  template <bool kWithV>
+  AFD_DEVICE void load(uint32_t stage, int64_t row, int lane) const {
+    using R = Ring<D>;
+    constexpr int kChunks = D / 32;  // 16-byte chunks of a row of codes
+#pragma unroll
+    for (int u = 0; u < kTile * kChunks / 32; ++u) {
+      const int i = u * 32 + lane;
+      const int r = i / kChunks, c = i % kChunks;
+      const uint32_t dst = stage + r * (D / 2) + swz<D>(r, c) * 16;
+      cp16(dst, kc + row * (D / 2) + i * 16);
+      if (kWithV) cp16(dst + R::kHalf, vc + row * (D / 2) + i * 16);
+    }
+    constexpr int kPairChunks = R::kPairs / 16;  // at most 16: K's by the lower half warp, V's by the upper
+    const int l = lane & 15;
+    if (l < kPairChunks && (kWithV || lane < 16))
+      cp16(stage + (lane < 16 ? 0 : R::kHalf) + R::kCodes + l * 16,
+           (lane < 16 ? ks : vs) + row * (D / kGroup) * 4 + l * 16);
+  }
+};
+
+// The query heads of one chunk as B operands, and their sums per dim group.
+// Column n of tile t is head t * 8 + n of the chunk (zero beyond `heads`).
+template <typename T, int D, int NT>
+struct Query {
+  static constexpr int G = D / kGroup;
+  uint32_t f[NT][G * 4][2];
+  float sum[NT][G][2];  // of heads 2c, 2c + 1, times scale * log2(e)
+
+  AFD_DEVICE void load(const T* sq, float scale_log2, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const T* row = sq + (t * 8 + g) * D + c * 16;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        float acc = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // word k / 2, half k % 2
+          const T* at = row + j * kGroup + (k >> 1) * 8 + (k & 1) * 2;
+          const T v[4] = {at[0], at[4], at[1], at[5]};
+          f[t][j * 4 + k][0] = reinterpret_cast<const uint16_t&>(v[0]) |
+                               (uint32_t) reinterpret_cast<const uint16_t&>(v[1]) << 16;
+          f[t][j * 4 + k][1] = reinterpret_cast<const uint16_t&>(v[2]) |
+                               (uint32_t) reinterpret_cast<const uint16_t&>(v[3]) << 16;
+          acc += (to_f32(v[0]) + to_f32(v[1])) + (to_f32(v[2]) + to_f32(v[3]));
+        }
+        acc += __shfl_xor_sync(0xffffffffu, acc, 1);
+        acc += __shfl_xor_sync(0xffffffffu, acc, 2);
+        acc *= scale_log2;
+        sum[t][j][0] = __shfl_sync(0xffffffffu, acc, c * 8);
+        sum[t][j][1] = __shfl_sync(0xffffffffu, acc, c * 8 + 4);
+      }
+    }
+  }
+};
+
+// s[t][i] for this lane: rows tile_row(g) (i = 0, 1) and tile_row(g) + 8
+// (i = 2, 3), heads t * 8 + 2c + (i & 1); in the log2 domain.
+template <typename T, int D, int NT>
+AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_t stage, float scale_log2, int lane) {
+  using R = Ring<D>;
+  constexpr int G = D / kGroup;
+  const int c = lane & 3, r0 = tile_row(lane >> 2);
+  const uint32_t pairs = stage + R::kCodes;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    uint32_t w0[2], w1[2];
+    const int chunk = 2 * j + (c >> 1);
+    lds64(w0[0], w0[1], stage + r0 * (D / 2) + swz<D>(r0, chunk) * 16 + (c & 1) * 8);
+    lds64(w1[0], w1[1], stage + (r0 + 8) * (D / 2) + swz<D>(r0 + 8, chunk) * 16 + (c & 1) * 8);
+    float acc[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t x = w0[k >> 1] >> ((k & 1) * 8), y = w1[k >> 1] >> ((k & 1) * 8);
+      const uint32_t a0 = Codes<T>::pair(x), a2 = Codes<T>::pair(x >> 4);
+      const uint32_t a1 = Codes<T>::pair(y), a3 = Codes<T>::pair(y >> 4);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mma<T>(acc[t], a0, a1, a2, a3, q.f[t][j * 4 + k][0], q.f[t][j * 4 + k][1]);
+    }
+    const uint32_t p0 = lds32(pairs + (r0 * G + j) * 4), p1 = lds32(pairs + ((r0 + 8) * G + j) * 4);
+    const float st0 = pair_step(p0), st1 = pair_step(p1);
+    const float z0 = fmaf(8.f, st0, pair_zero(p0)), z1 = fmaf(8.f, st1, pair_zero(p1));
+    const float m0 = st0 * scale_log2, m1 = st1 * scale_log2;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s[t][0] += fmaf(m0, acc[t][0], z0 * q.sum[t][j][0]);
+      s[t][1] += fmaf(m0, acc[t][1], z0 * q.sum[t][j][1]);
+      s[t][2] += fmaf(m1, acc[t][2], z1 * q.sum[t][j][0]);
+      s[t][3] += fmaf(m1, acc[t][3], z1 * q.sum[t][j][1]);
+    }
+  }
+}
+
+// Stage the chunk's query heads in shared memory (rows beyond them zero).
+template <typename T, int D, int NT>
+AFD_DEVICE void stage_query(T* sq, const Kv4DecodeParams& p, int b, int head0, int heads) {
+  const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + head0 * p.q_sh;
+  for (int i = threadIdx.x; i < NT * 8 * D; i += blockDim.x) {
+    const int h = i / D;
+    sq[i] = h < heads ? q[h * p.q_sh + i % D] : from_f32<T>(0.f);
+  }
+}
+
+// Unnormalised result of a piece in shared memory -> output or partial.
+template <typename T, int D, int NT>
+AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int heads, int64_t slot, bool whole,
+                             const float* red, const float* ml, int nact) {
+  // ml: [kWarps][NT * 8] maxima, then sums; red: [nact][NT * 8][D], already on the common maximum
+  constexpr int H = NT * 8;
+  for (int i = threadIdx.x; i < heads * (D / 4); i += kDecThreads) {
+    const int h = i / (D / 4), d4 = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    for (int w = 0; w < nact; ++w) m = fmaxf(m, ml[w * H + h]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < nact; ++w) {
+      const float f = m == -INFINITY ? 1.f : fast_exp2(ml[w * H + h] - m);
+      l = fmaf(ml[(kWarps + w) * H + h], f, l);
+      const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)w * H + h) * D + d4);
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    }
+    if (whole) {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head0 + h) * D + d4;
+      out[0] = from_f32<T>(o.x * inv);
+      out[1] = from_f32<T>(o.y * inv);
+      out[2] = from_f32<T>(o.z * inv);
+      out[3] = from_f32<T>(o.w * inv);
+      if (d4 == 0 && p.lse != nullptr)
+        p.lse[(int64_t)b * p.heads + head0 + h] = (m + log2f(l)) * 0.6931471805599453f;
+    } else {
+      *reinterpret_cast<float4*>(p.part_o + (slot * H + h) * D + d4) = o;
+      if (d4 == 0) {
+        p.part_ml[(slot * H + h) * 2] = m;
+        p.part_ml[(slot * H + h) * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+template <typename T, int D, int NT, int kStages>
+__global__ void __launch_bounds__(kDecThreads, (D * NT <= 128 ? 2 : 1)) decode_kernel(Kv4DecodeParams p) {
+  using R = Ring<D>;
+  constexpr int G = D / kGroup, H = NT * 8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_warp[kWarps];
+  __shared__ float s_ml[2 * kWarps * H];
+  uint8_t* ring = smem;  // reused by the warps' results once a piece is done
+  T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
+  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int heads_v = p.kv_heads * p.chunks;
+
+  int64_t at, end;
+  if (p.direct) {
+    at = 0;  // one (sequence, head chunk) per CTA
+    end = 1;
+  } else {
+    tile_prefix(p, cum, s_warp);
+    const int64_t total = (int64_t)cum[p.batch] * heads_v;
+    const int64_t per = tiles_per_cta(total, gridDim.x);
+    at = min(total, blockIdx.x * per);
+    end = min(total, at + per);
+  }
+  const int64_t first = at;
+  while (at < end) {
+    Piece pc;
+    if (p.direct) {
+      pc.b = blockIdx.x / heads_v;
+      pc.hv = blockIdx.x % heads_v;
+      pc.t0 = 0;
+      pc.t1 = (seq_len_of(p, pc.b) + kTile - 1) / kTile;
+      pc.whole = true;
+      at = end;
+    } else {
+      pc = piece_at(cum, p.batch, heads_v, at, end);
+    }
+    const int n = seq_len_of(p, pc.b);
+    const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
+    const int h_in = pc.hv % p.chunks * H;
+    const int heads = min(H, group - h_in);
+    const int head0 = kv_head * group + h_in;
+    const TileSource<D> src(p, pc.b, kv_head);
+    const uint32_t base = smem_u32(ring) + warp * kStages * R::kStageBytes;
+
+    // Fill the ring.  Tiles of a piece are dealt to the warps in turn.
+    int issue = pc.t0 + warp;
+    int64_t row = issue < pc.t1 ? src.row_of(issue) : 0;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (issue < pc.t1) {
+        src.template load<true>(base + s * R::kStageBytes, row, lane);
+        issue += kWarps;
+        if (issue < pc.t1) row = src.row_of(issue);
+      }
+      cp_commit();
+    }
+    stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
+    __syncthreads();
+    Query<T, D, NT> q;
+    q.load(sq, p.scale_log2, lane);
+
+    float o[NT][G * 4][4], zo[NT][G][2], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < G * 4; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < G; ++j) zo[t][j][0] = zo[t][j][1] = 0.f;
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+    }
+
+    int stage = 0;
+    const int r0 = tile_row(g);
+    for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      {  // refill the stage that the previous tile has left
+        const int into = stage == 0 ? kStages - 1 : stage - 1;
+        if (issue < pc.t1) {
+          src.template load<true>(base + into * R::kStageBytes, row, lane);
+          issue += kWarps;
+          if (issue < pc.t1) row = src.row_of(issue);
+        }
+        cp_commit();
+      }
+      const uint32_t st = base + stage * R::kStageBytes;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+
+      float s[NT][4];
+      tile_logits<T, D, NT>(s, q, st, p.scale_log2, lane);
+      const bool in0 = tile * kTile + r0 < n, in1 = tile * kTile + r0 + 8 < n;
+      bool grow = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (!in0) s[t][0] = s[t][1] = -INFINITY;
+        if (!in1) s[t][2] = s[t][3] = -INFINITY;
+        grow |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kLazy || fmaxf(s[t][1], s[t][3]) > m[t][1] + kLazy;
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[t][e], s[t][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(mx, m[t][e]);
+            const float f = mx == -INFINITY ? 1.f : fast_exp2(m[t][e] - mx);
+            m[t][e] = mx;
+            l[t][e] *= f;
+#pragma unroll
+            for (int j = 0; j < G; ++j) zo[t][j][e] *= f;
+#pragma unroll
+            for (int i = 0; i < G * 4; ++i) {
+              o[t][i][e] *= f;
+              o[t][i][2 + e] *= f;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float mm = m[t][i & 1];
+          s[t][i] = fast_exp2(s[t][i] - (mm == -INFINITY ? 0.f : mm));
+          l[t][i & 1] += s[t][i];
+        }
+      }
+      // P V: the probabilities, scaled per dim group, are the B operand.
+      const uint32_t pairs = st + R::kHalf + R::kCodes;
+      const uint32_t vbase = st + R::kHalf + (g & 3) * 4;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const uint32_t p0 = lds32(pairs + (r0 * G + j) * 4), p1 = lds32(pairs + ((r0 + 8) * G + j) * 4);
+        // positions past the end hold anything: their factors are zero, not 0 * that
+        const float st0 = in0 ? pair_step(p0) : 0.f, st1 = in1 ? pair_step(p1) : 0.f;
+        const float z0 = in0 ? fmaf(8.f, st0, pair_zero(p0)) : 0.f, z1 = in1 ? fmaf(8.f, st1, pair_zero(p1)) : 0.f;
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          zo[t][j][0] = fmaf(s[t][0], z0, fmaf(s[t][2], z1, zo[t][j][0]));
+          zo[t][j][1] = fmaf(s[t][1], z0, fmaf(s[t][3], z1, zo[t][j][1]));
+          b[t][0] = transpose8(pack_bf16(s[t][0] * st0, s[t][1] * st0));
+          b[t][1] = transpose8(pack_bf16(s[t][2] * st1, s[t][3] * st1));
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // k indices 2c, 2c + 1, 2c + 8, 2c + 9
+          const int r = tile_row(2 * c + (i & 1)) + (i >> 1) * 8;
+          w[i] = lds32(vbase + r * (D / 2) + swz<D>(r, 2 * j + (g >> 2)) * 16);
+        }
+        const uint32_t a = __byte_perm(w[0], w[1], 0x5410), bb = __byte_perm(w[0], w[1], 0x7632);
+        const uint32_t cc = __byte_perm(w[2], w[3], 0x5410), dd = __byte_perm(w[2], w[3], 0x7632);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a0 = Codes<__nv_bfloat16>::pair(a >> (4 * i)), a1 = Codes<__nv_bfloat16>::pair(bb >> (4 * i));
+          const uint32_t a2 = Codes<__nv_bfloat16>::pair(cc >> (4 * i)), a3 = Codes<__nv_bfloat16>::pair(dd >> (4 * i));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma<__nv_bfloat16>(o[t][j * 4 + i], a0, a1, a2, a3, b[t][0], b[t][1]);
+        }
+      }
+      __syncwarp();  // every lane is done with this stage before it is refilled
+    }
+    cp_wait<0>();
+    __syncthreads();  // the ring is free: it takes the warps' results
+
+    const int nact = min(kWarps, pc.t1 - pc.t0);
+    float* red = reinterpret_cast<float*>(ring);
+    if (warp < nact) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float ls = l[t][e], z[G];
+#pragma unroll
+          for (int j = 0; j < G; ++j) z[j] = zo[t][j][e];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            ls += __shfl_xor_sync(0xffffffffu, ls, x);
+#pragma unroll
+            for (int j = 0; j < G; ++j) z[j] += __shfl_xor_sync(0xffffffffu, z[j], x);
+          }
+          const int h = t * 8 + 2 * c + e;
+          if (g == 0) {
+            s_ml[warp * H + h] = m[t][e];
+            s_ml[(kWarps + warp) * H + h] = ls;
+          }
+          float* to = red + ((size_t)warp * H + h) * D + g * 8;
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            *reinterpret_cast<float4*>(to + j * kGroup) =
+                make_float4(o[t][j * 4][e] + z[j], o[t][j * 4 + 1][e] + z[j], o[t][j * 4 + 2][e] + z[j],
+                            o[t][j * 4 + 3][e] + z[j]);
+            *reinterpret_cast<float4*>(to + j * kGroup + 4) =
+                make_float4(o[t][j * 4][2 + e] + z[j], o[t][j * 4 + 1][2 + e] + z[j], o[t][j * 4 + 2][2 + e] + z[j],
+                            o[t][j * 4 + 3][2 + e] + z[j]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    // A CTA's first piece starts its share, its last ends it: two partial slots each.
+    write_result<T, D, NT>(p, pc.b, head0, heads, 2 * (int64_t)blockIdx.x + (at == first ? 0 : 1), pc.whole, red, s_ml,
+                           nact);
+    __syncthreads();
+    if (!p.direct) at += pc.t1 - pc.t0;
+  }
+}
+
+// Joins the partials of every (sequence, head) that more than one CTA worked
+// on, and writes the empty sequences.  One block per (sequence, query head).
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, int heads_chunk, int ctas) {
+  __shared__ int s_sum[2][4];
+  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < p.batch; i += blockDim.x) {
+    const int t = (seq_len_of(p, i) + kTile - 1) / kTile;
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[0][threadIdx.x / 32] = before;
+    s_sum[1][threadIdx.x / 32] = all;
+  }
+  __syncthreads();
+  before = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
+  all = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
+  const int tiles = (seq_len_of(p, b) + kTile - 1) / kTile;
+  T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head) * dim;
+  pdl_wait();
+  if (tiles == 0) {
+    for (int d = threadIdx.x; d < dim; d += blockDim.x) out[d] = from_f32<T>(0.f);
+    if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = -INFINITY;
+    return;
+  }
+  const int group = p.heads / p.kv_heads;
+  const int kv_head = head / group, hc = head % group / heads_chunk, h = head % group % heads_chunk;
+  const int heads_v = p.kv_heads * p.chunks;
+  const int64_t per = tiles_per_cta((int64_t)all * heads_v, ctas);
+  const int64_t start = (int64_t)before * heads_v + (int64_t)(kv_head * p.chunks + hc) * tiles;
+  const int64_t c0 = start / per, c1 = (start + tiles - 1) / per;
+  if (c0 == c1) return;  // one CTA had all of it and wrote the result
+  auto slot = [&](int64_t c) { return (2 * c + (c == c0 && start != c0 * per ? 1 : 0)) * heads_chunk + h; };
+  float m = -INFINITY;
+  for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, p.part_ml[slot(c) * 2]);
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  const int d0 = threadIdx.x, d1 = threadIdx.x + 128;
+#pragma unroll 4
+  for (int64_t c = c0; c <= c1; ++c) {
+    const int64_t sl = slot(c);
+    const float f = m == -INFINITY ? 1.f : fast_exp2(p.part_ml[sl * 2] - m);
+    l = fmaf(p.part_ml[sl * 2 + 1], f, l);
+    if (d0 < dim) o0 = fmaf(p.part_o[sl * dim + d0], f, o0);
+    if (d1 < dim) o1 = fmaf(p.part_o[sl * dim + d1], f, o1);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (d0 < dim) out[d0] = from_f32<T>(o0 * inv);
+  if (d1 < dim) out[d1] = from_f32<T>(o1 * inv);
+  if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// Adds every position's probability to its score.  The same shares of tiles;
+// nothing to merge, since a position is in one tile.
+template <typename T, int D, int NT, int kStages>
+__global__ void __launch_bounds__(kDecThreads, 2) score_kernel(Kv4DecodeParams p) {
+  using R = Ring<D>;
+  constexpr int H = NT * 8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_warp[kWarps];
+  T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
+  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int c = lane & 3;
+  const int heads_v = p.kv_heads * p.chunks;
+  tile_prefix(p, cum, s_warp);
+  const int64_t total = (int64_t)cum[p.batch] * heads_v;
+  const int64_t per = tiles_per_cta(total, gridDim.x);
+  int64_t at = min(total, blockIdx.x * per);
+  const int64_t end = min(total, at + per);
+  pdl_wait();  // the log-sum-exps of the decode
+  while (at < end) {
+    const Piece pc = piece_at(cum, p.batch, heads_v, at, end);
+    const int n = seq_len_of(p, pc.b);
+    const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
+    const int h_in = pc.hv % p.chunks * H;
+    const int heads = min(H, group - h_in);
+    const int head0 = kv_head * group + h_in;
+    const TileSource<D> src(p, pc.b, kv_head);
+    const uint32_t base = smem_u32(smem) + warp * kStages * R::kHalf;
+    int issue = pc.t0 + warp;
+    int64_t row = issue < pc.t1 ? src.row_of(issue) : 0;
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (issue < pc.t1) {
+        src.template load<false>(base + s * R::kHalf, row, lane);
+        issue += kWarps;
+        if (issue < pc.t1) row = src.row_of(issue);
+      }
+      cp_commit();
+    }
+    stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
+    __syncthreads();
+    Query<T, D, NT> q;
+    q.load(sq, p.scale_log2, lane);
+    float lse[NT][2];  // log2 domain; heads beyond the group and empty rows weigh nothing
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = t * 8 + 2 * c + e;
+        lse[t][e] = h < heads ? p.lse[(int64_t)pc.b * p.heads + head0 + h] * 1.4426950408889634f : INFINITY;
+      }
+    int stage = 0;
+    const int r0 = tile_row(lane >> 2);
+    for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      {
+        const int into = stage == 0 ? kStages - 1 : stage - 1;
+        if (issue < pc.t1) {
+          src.template load<false>(base + into * R::kHalf, row, lane);
+          issue += kWarps;
+          if (issue < pc.t1) row = src.row_of(issue);
+        }
+        cp_commit();
+      }
+      float s[NT][4];
+      tile_logits<T, D, NT>(s, q, base + stage * R::kHalf, p.scale_log2, lane);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      float w0 = 0.f, w1 = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        w0 += fast_exp2(s[t][0] - lse[t][0]) + fast_exp2(s[t][1] - lse[t][1]);
+        w1 += fast_exp2(s[t][2] - lse[t][0]) + fast_exp2(s[t][3] - lse[t][1]);
+      }
+      w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+      w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
+      w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+      w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
+      // Adds, not stores: head chunks and sequences that share blocks meet here.
+      if (c < 2) {
+        const int r = r0 + c * 8;
+        if (tile * kTile + r < n) atomicAdd(p.scores + src.row_of(tile) + r, c == 0 ? w0 : w1);
+      }
+      __syncwarp();
+    }
+    cp_wait<0>();
+    __syncthreads();
+    at += pc.t1 - pc.t0;
+  }
+}
+
+template <typename T, int D, int NT, int kStages>
+cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
+  constexpr int H = NT * 8;
+  const int ring = kWarps * kStages * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
+  p.ring_bytes = ring > red ? ring : red;
+  const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.direct ? 0 : (p.batch + 1) * 4);
+  static PerDeviceOnce attr;
+  cudaError_t e = attr.run([&] {
+    return cudaFuncSetAttribute(decode_kernel<T, D, NT, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
+  });
+  if (e != cudaSuccess) return e;
+  decode_kernel<T, D, NT, kStages><<<p.ctas, kDecThreads, smem, s>>>(p);
+  if (!p.direct) {
+    e = launch_pdl(join_kernel<T>, dim3((unsigned)(p.batch * p.heads)), dim3(128), 0, s, p, D, H, p.ctas);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaGetLastError();
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch_score(Kv4DecodeParams p, cudaStream_t s) {
+  constexpr int kStages = 4, H = NT * 8;
+  p.ring_bytes = kWarps * kStages * Ring<D>::kHalf;
+  const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.batch + 1) * 4;
+  static PerDeviceOnce attr;
+  cudaError_t e = attr.run([&] {
+    return cudaFuncSetAttribute(score_kernel<T, D, NT, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(score_kernel<T, D, NT, kStages>, dim3(2 * device_sm_count()), dim3(kDecThreads), (size_t)smem, s,
+                    p);
+}
+
+template <typename T, int D, int NT>
+cudaError_t run(const Kv4DecodeParams& p, cudaStream_t s) {
+  const cudaError_t e = launch_decode<T, D, NT, 4>(p, s);
+  if (e != cudaSuccess || p.scores == nullptr) return e;
+  return launch_score<T, D, NT>(p, s);
+}
+
+template <typename T>
+cudaError_t dispatch(const Kv4DecodeParams& p, cudaStream_t s) {
+  const bool wide = p.head_tiles == 2;
+  switch (p.dim) {
+    case 64: return wide ? run<T, 64, 2>(p, s) : run<T, 64, 1>(p, s);
+    case 128: return wide ? run<T, 128, 2>(p, s) : run<T, 128, 1>(p, s);
+    default: return run<T, 256, 1>(p, s);
+  }
+}
+
+}  // namespace kv4
+}  // namespace afd
+
+using namespace afd;
+
+Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len) {
+  Kv4Plan plan;
+  const int group = heads / kv_heads;
+  // 16 heads share one unpacking of the codes; at D = 256 their accumulators
+  // would not fit in registers, so wider groups take chunks of 8.
+  plan.head_tiles = dim <= 128 && group > 8 ? 2 : 1;
+  const int per = 8 * plan.head_tiles;
+  plan.chunks = (group + per - 1) / per;
+  const int64_t items = (int64_t)batch * kv_heads * plan.chunks;
+  constexpr int kDirectTiles = 32;
+  plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
+  const int resident = dim * plan.head_tiles <= 128 ? 2 : 1;
+  plan.ctas = plan.direct ? (int)items : resident * device_sm_count();
+  plan.max_batch = kv4::kMaxBatch;
+  return plan;
+}
+
+int launch_gqa_decode_int4(const Kv4DecodeParams& p, int dtype, cudaStream_t s) {
+  return (int)(dtype == kF16 ? kv4::dispatch<__half>(p, s) : kv4::dispatch<__nv_bfloat16>(p, s));
+}

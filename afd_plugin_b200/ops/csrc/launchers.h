@@ -362,3 +362,58 @@ struct GdnRecurrentParams {
 };
 void launch_gdn_conv(const GdnConvParams& p, cudaStream_t s);
 bool launch_gdn_recurrent(const GdnRecurrentParams& p, cudaStream_t s);
+
+// ---- kv_int4.cu / gqa_decode_int4.cu (cache layout: kv_int4.cuh)
+struct Kv4WriteParams {
+  const void *k, *v;          // [tokens, kv_heads, dim] with element strides, last dim dense
+  int64_t k_st, k_sh, v_st, v_sh;
+  const int64_t* slots;       // [tokens]
+  uint8_t *k_codes, *v_codes;
+  uint32_t *k_scale, *v_scale;
+  float* scores;              // [blocks, kv_heads, block_size] or null: set to zero at the written slots
+  int* status;
+  int64_t num_slots;
+  int tokens, kv_heads, dim, block_size;
+  int vec;                    // rows are 16-byte aligned
+};
+struct Kv4ReadParams {
+  void *k, *v;                // [tokens, kv_heads, dim]
+  const int64_t* slots;
+  const uint8_t *k_codes, *v_codes;
+  const uint32_t *k_scale, *v_scale;
+  int* status;
+  int64_t num_slots;
+  int tokens, kv_heads, dim, block_size;
+};
+void launch_kv4_write(const Kv4WriteParams& p, int dtype, cudaStream_t s);
+void launch_kv4_read(const Kv4ReadParams& p, int dtype, cudaStream_t s);
+
+struct Kv4DecodeParams {
+  const void* q;              // [batch, heads, dim], element strides q_sb / q_sh
+  int64_t q_sb, q_sh;
+  void* out;                  // [batch, heads, dim]
+  float* lse;                 // [batch, heads] natural log, or null
+  const uint8_t *k_codes, *v_codes;
+  const uint32_t *k_scale, *v_scale;
+  float* scores;              // [blocks, kv_heads, block_size] or null (needs lse)
+  const int32_t* block_table; // [batch, max_blocks], row stride table_stride
+  const int32_t* seq_lens;
+  int64_t table_stride;
+  float* part_o;              // [2 * ctas, 8 * head_tiles, dim] (not direct)
+  float* part_ml;             // [2 * ctas, 8 * head_tiles, 2]
+  int* status;                // or null
+  int batch, heads, kv_heads, dim, block_size, num_blocks, max_blocks;
+  int head_tiles, chunks, ctas, direct;  // from the plan
+  int ring_bytes;             // set by the launcher
+  float scale_log2;
+};
+struct Kv4Plan {
+  int head_tiles;  // 8 or 16 query heads of a KV head per pass
+  int chunks;      // passes that cover its whole group
+  int ctas;
+  int max_batch;   // sequences one launch takes
+  bool direct;     // one CTA per (sequence, head chunk), no partials
+};
+Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len);
+// Returns a cudaError_t.
+int launch_gqa_decode_int4(const Kv4DecodeParams& p, int dtype, cudaStream_t s);

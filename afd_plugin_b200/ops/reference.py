@@ -114,6 +114,120 @@ def apply_rope(
     return out.to(x.dtype)
 
 
+# ----------------------------------------------------------- 4-bit KV cache
+INT4_GROUP = 64  # dims that share one (step, zero)
+
+
+def int4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pack rows ``x [..., d]``: codes ``[..., d / 2]`` uint8 (dim ``2 i`` in the low nibble of byte
+    ``i``) and bf16 ``(step, zero) [..., d / 64, 2]``.
+
+    ``zero`` is the group's minimum rounded down to bf16, ``step`` is ``(max - zero) / 15`` rounded
+    up to bf16, and ``c = clamp(rint((x - zero) / step), 0, 15)``, in fp32 throughout: the stored
+    value ``zero + c * step`` is within half a step of ``x``.
+    """
+    g = x.float().unflatten(-1, (-1, INT4_GROUP))
+    lo = g.amin(-1, keepdim=True).contiguous()
+    bits = lo.view(torch.int32)  # cut to the upper 16 bits; a negative value grows in magnitude first
+    zero = (torch.where(bits < 0, bits + 0xFFFF, bits) & -0x10000).view(torch.float32)
+    step = (g.amax(-1, keepdim=True) - zero) / g.new_full((1,), 15.0)
+    step = ((step.contiguous().view(torch.int32) + 0xFFFF) & -0x10000).view(torch.float32)
+    c = torch.where(step > 0, (g - zero) / step, torch.zeros_like(g)).round().clamp(0, 15)
+    c = c.nan_to_num(0.0).to(torch.uint8).flatten(-2)
+    return c[..., 0::2] | (c[..., 1::2] << 4), torch.cat([step, zero], -1).bfloat16()
+
+
+def int4_dequantize(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """fp32 values of packed rows."""
+    c = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).float()
+    s = scale.float()
+    return (s[..., 1:] + c.unflatten(-1, (-1, INT4_GROUP)) * s[..., :1]).flatten(-2)
+
+
+def gqa_cache_write_int4(kv, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                         scores: torch.Tensor | None = None) -> None:
+    bs = kv.k.shape[2]
+    blk, off = slot_mapping.long() // bs, slot_mapping.long() % bs
+    kv.k[blk, :, off], kv.k_scale[blk, :, off] = int4_quantize(k)
+    kv.v[blk, :, off], kv.v_scale[blk, :, off] = int4_quantize(v)
+    if scores is not None:
+        scores[blk, :, off] = 0.0
+
+
+def gqa_cache_read_int4(kv, slots: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    bs = kv.k.shape[2]
+    blk, off = slots.long() // bs, slots.long() % bs
+    return (int4_dequantize(kv.k[blk, :, off], kv.k_scale[blk, :, off]).to(dtype),
+            int4_dequantize(kv.v[blk, :, off], kv.v_scale[blk, :, off]).to(dtype))
+
+
+def _int4_positions(block_row: torch.Tensor, n: int, block_size: int) -> torch.Tensor:
+    pos = torch.arange(n, device=block_row.device)
+    return block_row.long()[pos // block_size] * block_size + pos % block_size
+
+
+def gqa_decode_int4(q: torch.Tensor, kv, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                    scores: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(o [B, heads, d], lse [B, heads])``; an empty sequence gives zeros and ``-inf``."""
+    hkv, bs = kv.k.shape[1], kv.k.shape[2]
+    B, hq, d = q.shape
+    out = torch.zeros(B, hq, d, dtype=q.dtype, device=q.device)
+    lse = torch.full((B, hq), float("-inf"), device=q.device)
+    for b, n in enumerate(seq_lens.clamp(0, block_table.shape[1] * bs).tolist()):
+        if n == 0:
+            continue
+        slots = _int4_positions(block_table[b], n, bs)
+        k, v = gqa_cache_read_int4(kv, slots, torch.float32)  # [n, hkv, d]
+        s = torch.einsum("kgd,nkd->kgn", q[b].float().view(hkv, hq // hkv, d), k) * scale
+        lse[b] = torch.logsumexp(s, -1).flatten()
+        p = torch.softmax(s, -1)
+        out[b] = torch.einsum("kgn,nkd->kgd", p, v).reshape(hq, d).to(q.dtype)
+        if scores is not None:
+            blk, off = slots // bs, slots % bs
+            scores.index_put_((blk[None, :], torch.arange(hkv, device=q.device)[:, None], off[None, :]), p.sum(1),
+                              accumulate=True)
+    return out, lse
+
+
+def kv_evict_int4(kv, scores: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int,
+                  recent: int) -> tuple[torch.Tensor, torch.Tensor]:
+    hkv, bs = scores.shape[1], scores.shape[2]
+    B = seq_lens.shape[0]
+    kept = torch.full((B, hkv, budget), -1, dtype=torch.int32, device=scores.device)
+    for b, n in enumerate(seq_lens.tolist()):
+        n = max(n, 0)
+        if n <= budget:
+            kept[b, :, :n] = torch.arange(n, dtype=torch.int32, device=scores.device)
+            continue
+        slots = _int4_positions(block_table[b], n, bs)
+        blk, off = slots // bs, slots % bs
+        for h in range(hkv):
+            key = scores[blk, h, off][: n - recent]
+            key = torch.where(key.isnan(), float("-inf"), key)
+            best = torch.sort(key, descending=True, stable=True).indices[: budget - recent]
+            keep = torch.cat([best, torch.arange(n - recent, n, device=best.device)]).sort().values
+            kept[b, h] = keep.int()
+            for t in (*kv, scores):
+                t[blk[:budget], h, off[:budget]] = t[blk[keep], h, off[keep]]
+    return seq_lens.clamp(0, budget).to(torch.int32), kept
+
+
+# ------------------------------------------------------------- int8 linear
+def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows to int8 with one fp32 scale each: ``q = clamp(rint(x * (127 / amax)), -127, 127)``,
+    ``scale = amax / 127``, ``amax = max(|x|, 2^-100)``."""
+    amax = x.float().abs().amax(-1, keepdim=True).clamp(min=2.0**-100)
+    top = amax.new_full((1,), 127.0)
+    q = (x.float() * (top / amax)).round().clamp(-127, 127).nan_to_num(0.0).to(torch.int8)
+    return q, (amax / top).squeeze(-1)
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+    q, s = int8_quantize(x)
+    acc = q.double() @ w.double().t()  # whole numbers below 2^53: exact
+    return (acc.float() * (s[:, None] * w_scale.float()[None, :])).to(out_dtype)
+
+
 # ------------------------------------------------------------------ routing
 def topk_route(
     logits: torch.Tensor,
