@@ -390,6 +390,35 @@ def gqa_decode_int4(
     return (out, lse) if return_lse else out
 
 
+def kv_evict_int4(
+    kv: Int4KV,
+    scores: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    budget: int,
+    recent: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence longer than ``budget`` to ``budget`` cached positions, in place.
+
+    Each KV head keeps the last ``recent`` positions and the ``budget - recent`` others with the
+    largest ``scores`` (ties: the earlier position; NaN ranks as ``-inf``).  Kept rows move, in
+    order, to the sequence's first ``budget`` positions, their scores with them; rows behind those
+    stay as they were.  Returns the new lengths, int32 ``[B]``, and the positions kept, ascending,
+    int32 ``[B, kv_heads, budget]`` (-1 past a shorter sequence's end).  Sequences of one call must
+    not share blocks: a shared block would be compacted twice.
+    """
+    if checks.enabled():
+        checks.paged_attention("kv_evict_int4", block_table, seq_lens, num_blocks=kv.num_blocks,
+                               block_size=kv.block_size, min_len=0)
+    if _cuda(scores):
+        return _cuda_ops().kv_evict_int4(*kv, scores, block_table, seq_lens, budget, recent)
+    kv_int4.check_cache("kv_evict_int4", kv, scores)
+    kv_int4.check_batch("kv_evict_int4", block_table, seq_lens, seq_lens.shape[0])
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"kv_evict_int4: 1 <= budget and 0 <= recent <= budget, got {budget} and {recent}")
+    return ref.kv_evict_int4(kv, scores, block_table, seq_lens, budget, recent)
+
+
 # -------------------------------------------------------------------- MoE
 def moe_experts(
     x: torch.Tensor,
@@ -488,6 +517,7 @@ __all__ = [
     "gqa_decode_int4",
     "head_linear",
     "int4_kv_cache",
+    "kv_evict_int4",
     "linear",
     "mla_cache_write",
     "mla_decode",

@@ -667,6 +667,49 @@ std::tuple<at::Tensor, at::Tensor> gqa_decode_int4(const at::Tensor& q, const at
   return {out, lse};
 }
 
+std::tuple<at::Tensor, at::Tensor> kv_evict_int4(at::Tensor& kc, at::Tensor& ks, at::Tensor& vc, at::Tensor& vs,
+                                                 at::Tensor& scores, const at::Tensor& table, const at::Tensor& lens,
+                                                 int64_t budget, int64_t recent) {
+  const char* op = "kv_evict_int4";
+  check_cuda(kc, "the cache");
+  const Kv4Shape sh = check_kv4(kc, ks, vc, vs, op);
+  Kv4EvictParams p{};
+  p.scores = check_kv4_scores(scores, kc, op);
+  const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
+  check_kv4_batch(table, lens, kc, B, op);
+  TORCH_CHECK(budget >= 1 && budget <= INT32_MAX && recent >= 0 && recent <= budget, op,
+              ": 1 <= budget and 0 <= recent <= budget");
+  TORCH_CHECK(B * sh.kv_heads <= (1 << 27), op, ": too many sequences");
+  c10::cuda::CUDAGuard g(kc.device());
+  auto new_lens = at::empty({B}, lens.options());
+  auto kept = at::empty({B, sh.kv_heads, budget}, lens.options());
+  if (B == 0) return {new_lens, kept};
+  if (table.size(1) == 0) {
+    new_lens.zero_();
+    kept.fill_(-1);
+    return {new_lens, kept};
+  }
+  p.k_codes = kc.data_ptr<uint8_t>();
+  p.v_codes = vc.data_ptr<uint8_t>();
+  p.k_scale = reinterpret_cast<uint32_t*>(ks.data_ptr());
+  p.v_scale = reinterpret_cast<uint32_t*>(vs.data_ptr());
+  p.block_table = table.data_ptr<int32_t>();
+  p.seq_lens = lens.data_ptr<int32_t>();
+  p.new_lens = new_lens.data_ptr<int32_t>();
+  p.kept = kept.data_ptr<int32_t>();
+  p.table_stride = table.stride(0);
+  p.status = status_ptr_or_null(kc);
+  p.batch = (int)B;
+  p.kv_heads = sh.kv_heads;
+  p.block_size = sh.block_size;
+  p.num_blocks = sh.blocks;
+  p.max_blocks = (int)table.size(1);
+  p.budget = (int)budget;
+  p.recent = (int)recent;
+  C10_CUDA_CHECK((cudaError_t)launch_kv_evict_int4(p, sh.dim, stream()));
+  return {new_lens, kept};
+}
+
 // -------------------------------------------------------------------- MoE
 std::vector<at::Tensor> moe_align(const at::Tensor& topk_ids, int64_t e_local, int64_t offset, int64_t n_shared) {
   check_cuda(topk_ids, "topk_ids");
@@ -1389,6 +1432,8 @@ TORCH_LIBRARY(afd_b200, m) {
         "(Tensor, Tensor)");
   m.def("gqa_decode_int4(Tensor q, Tensor kc, Tensor ks, Tensor vc, Tensor vs, Tensor block_table, Tensor seq_lens, "
         "float scale, Tensor(a!)? scores, bool return_lse) -> (Tensor, Tensor)");
+  m.def("kv_evict_int4(Tensor(a!) kc, Tensor(b!) ks, Tensor(c!) vc, Tensor(d!) vs, Tensor(e!) scores, "
+        "Tensor block_table, Tensor seq_lens, int budget, int recent) -> (Tensor, Tensor)");
   m.def("moe_align(Tensor topk_ids, int e_local, int offset, int n_shared) -> Tensor[]");
   m.def("moe_gather(Tensor x, Tensor row_token, Tensor total) -> Tensor");
   m.def("grouped_gemm(Tensor a, Tensor w, Tensor offsets, Tensor counts, int epilogue) -> Tensor");
@@ -1451,6 +1496,7 @@ TORCH_LIBRARY_IMPL(afd_b200, CUDA, m) {
   m.impl("gqa_cache_write_int4", &gqa_cache_write_int4);
   m.impl("gqa_cache_read_int4", &gqa_cache_read_int4);
   m.impl("gqa_decode_int4", &gqa_decode_int4);
+  m.impl("kv_evict_int4", &kv_evict_int4);
   m.impl("moe_align", &moe_align);
   m.impl("moe_gather", &moe_gather);
   m.impl("grouped_gemm", &grouped_gemm);

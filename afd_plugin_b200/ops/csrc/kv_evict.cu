@@ -1,0 +1,282 @@
+// Eviction from the paged 4-bit KV cache by accumulated attention weight.
+//
+// A sequence of n > budget positions keeps, for each KV head, its last
+// `recent` positions and the budget - recent best scored of the others (ties
+// go to the earlier position).  The kept rows move, in order, to the
+// sequence's first `budget` positions, in place; the scores move with them.
+//
+// One cluster of CTAs works on one (sequence, KV head):
+//   1. the CTAs take equal runs of positions and turn scores into 32-bit keys
+//      that order like the scores (in shared memory, as far as they fit);
+//   2. four passes over 8 bits each find the key of the last kept position:
+//      shared-memory histograms, summed over the cluster through distributed
+//      shared memory;
+//   3. each warp counts its run, a prefix over warps and CTAs gives every kept
+//      position its rank;
+//   4. rows move in chunks: all CTAs load a chunk into registers, a cluster
+//      barrier, then they store it.  Row i comes from a position >= i, so a
+//      chunk's stores only overwrite rows that this chunk or an earlier one
+//      has loaded, and the next chunk's loads are issued before the barrier.
+//
+// What bounds it: the moved rows, read and written once (148 B each way at
+// D = 128), and one read of the scores.  The cluster size spreads small
+// batches over the SMs.
+#include <cooperative_groups.h>
+
+#include "device_state.h"
+#include "kv_int4.cuh"
+#include "launchers.h"
+
+namespace afd {
+namespace kv4 {
+namespace cg = cooperative_groups;
+
+constexpr int kEvThreads = 512;
+constexpr int kEvWarps = kEvThreads / 32;
+constexpr int kUnits = 4;  // 16-byte units of codes a thread moves per chunk
+
+// Orders like the float; NaN counts as -inf, -0 as 0.
+AFD_DEVICE uint32_t order_key(float x) {
+  if (x != x) x = -INFINITY;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+struct EvictView {
+  const Kv4EvictParams& p;
+  const int32_t* table;
+  int64_t head_off, block_rows;
+  AFD_DEVICE EvictView(const Kv4EvictParams& q, int b, int h)
+      : p(q), table(q.block_table + (int64_t)b * q.table_stride), head_off((int64_t)h * q.block_size),
+        block_rows((int64_t)q.kv_heads * q.block_size) {}
+  // Cache row of a position.  A block id outside the pool is reported and replaced by the padding block.
+  AFD_DEVICE int64_t row(int pos) const {
+    const int pg = pos / p.block_size;
+    int blk = table[pg];
+    if ((unsigned)blk >= (unsigned)p.num_blocks) {
+      if (p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
+      blk = 0;
+    }
+    return blk * block_rows + head_off + (pos - pg * p.block_size);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
+  constexpr int G = D / kGroup;
+  constexpr int kRowUnits = 2 * D / 32;                     // 16-byte units of codes of a row, K then V
+  constexpr int kRows = kUnits * kEvThreads / kRowUnits;    // rows a CTA moves per chunk
+  constexpr int kRowWords = 2 * G + 1;                      // (step, zero) pairs of K and V, and the score
+  constexpr int kWords = (kRows * kRowWords + kEvThreads - 1) / kEvThreads;
+  extern __shared__ uint32_t s_keys[];
+  __shared__ uint32_t s_hist[2][256];
+  __shared__ uint32_t s_pick[2];              // digit, positions still to take from it
+  __shared__ int s_warp[2][kEvWarps];         // kept-for-sure / tied positions of each warp's run
+  __shared__ int s_cta[2];                    // the CTA's totals, read by the others
+  __shared__ uint32_t s_scan[8];
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int item = blockIdx.x / cs;
+  const int b = item / p.kv_heads, h = item % p.kv_heads;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  int n = p.seq_lens[b];
+  n = n < 0 ? 0 : min(n, p.max_blocks * p.block_size);
+  int32_t* kept = p.kept + (int64_t)item * p.budget;
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = min(n, p.budget);
+  if (n <= p.budget) {  // the same for the whole cluster
+    for (int i = rank * kEvThreads + tid; i < p.budget; i += cs * kEvThreads) kept[i] = i < n ? i : -1;
+    return;
+  }
+  const EvictView view(p, b, h);
+  const int m = n - p.recent;             // candidates
+  const int need = p.budget - p.recent;   // of them to keep: 0 <= need < m
+  const int per = (m + cs - 1) / cs;
+  const int lo = min(m, rank * per), cnt = min(m, lo + per) - lo;
+
+  auto load_key = [&](int i) { return order_key(p.scores[view.row(lo + i)]); };
+  for (int i = tid; i < min(cnt, p.key_cap); i += kEvThreads) s_keys[i] = load_key(i);
+  auto key_at = [&](int i) { return i < p.key_cap ? s_keys[i] : load_key(i); };
+  for (int i = tid; i < 2 * 256; i += kEvThreads) (&s_hist[0][0])[i] = 0;
+  __syncthreads();
+
+  // The key of the last position kept (`bound`) and how many of its ties are.
+  uint32_t bound = 0, left = (uint32_t)need;
+  const int padded = (cnt + 31) & ~31;
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    uint32_t* hist = s_hist[pass & 1];
+    for (int i = tid; i < padded; i += kEvThreads) {  // whole warps enter
+      const uint32_t key = i < cnt ? key_at(i) : 0;
+      const bool in = i < cnt && (pass == 0 || (key >> (shift + 8)) == (bound >> (shift + 8)));
+      const uint32_t digit = (key >> shift) & 255u;
+      // Scores crowd in few exponents: one add where a warp agrees.
+      const uint32_t act = __ballot_sync(0xffffffffu, in);
+      if (act == 0) continue;
+      const uint32_t first = __shfl_sync(0xffffffffu, digit, __ffs(act) - 1);
+      if (__all_sync(0xffffffffu, !in || digit == first)) {
+        if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popc(act));
+      } else if (in) {
+        atomicAdd(&hist[digit], 1u);
+      }
+    }
+    cluster.sync();
+    uint32_t sum = 0, above = 0;
+    if (tid < 256) {  // thread t looks at digit 255 - t: descending order
+      for (int r = 0; r < cs; ++r) sum += cluster.map_shared_rank(hist, r)[255 - tid];
+      above = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, above, o);
+        if (lane >= o) above += u;
+      }
+      if (lane == 31) s_scan[warp] = above;
+    }
+    __syncthreads();
+    if (tid < 256) {
+      for (int w = 0; w < warp; ++w) above += s_scan[w];
+      above -= sum;  // positions with a higher digit
+      if (above < left && left <= above + sum) {
+        s_pick[0] = 255 - tid;
+        s_pick[1] = left - above;
+      }
+      if (left == 0 && tid == 0) {  // nothing to take: a bound above every key
+        s_pick[0] = 255;
+        s_pick[1] = 0;
+      }
+    }
+    // the other buffer was read before this pass's barrier: clear it for the next pass
+    if (tid >= 256) s_hist[(pass + 1) & 1][tid - 256] = 0;
+    __syncthreads();
+    bound |= s_pick[0] << shift;
+    left = s_pick[1];
+    __syncthreads();
+  }
+  // left = ties of `bound` to keep, the earliest ones (0 only when need is 0).
+  const bool none = need == 0;
+
+  // Each warp's run of positions: its sure and tied counts, then ranks.
+  const int seg = ((cnt + kEvWarps - 1) / kEvWarps + 31) & ~31;
+  const int w0 = min(cnt, warp * seg), w1 = min(cnt, w0 + seg);
+  int gt = 0, eq = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t key = key_at(i);
+    gt += !none && key > bound;
+    eq += !none && key == bound;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt += __shfl_xor_sync(0xffffffffu, gt, o);
+    eq += __shfl_xor_sync(0xffffffffu, eq, o);
+  }
+  if (lane == 0) {
+    s_warp[0][warp] = gt;
+    s_warp[1][warp] = eq;
+  }
+  __syncthreads();
+  int gt_before = 0, eq_before = 0;
+  for (int w = 0; w < warp; ++w) {
+    gt_before += s_warp[0][w];
+    eq_before += s_warp[1][w];
+  }
+  if (tid == kEvThreads - 1) {
+    s_cta[0] = gt_before + gt;
+    s_cta[1] = eq_before + eq;
+  }
+  cluster.sync();
+  for (int r = 0; r < rank; ++r) {
+    const int* other = cluster.map_shared_rank(s_cta, r);
+    gt_before += other[0];
+    eq_before += other[1];
+  }
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < w1 ? key_at(i) : 0;
+    const bool is_gt = i < w1 && !none && key > bound, is_eq = i < w1 && !none && key == bound;
+    const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+    const uint32_t below = (1u << lane) - 1;
+    const int eq_rank = eq_before + __popc(me & below);
+    if (is_gt || (is_eq && eq_rank < (int)left))
+      kept[gt_before + __popc(mg & below) + min(eq_rank, (int)left)] = lo + i;
+    gt_before += __popc(mg);
+    eq_before += __popc(me);
+  }
+  for (int i = rank * kEvThreads + tid; i < p.recent; i += cs * kEvThreads) kept[need + i] = m + i;
+  cluster.sync();  // the list is complete, and visible to the cluster
+
+  // Move.  16-byte units of codes and 4-byte words of pairs and scores.
+  uint4* const kc = reinterpret_cast<uint4*>(p.k_codes);
+  uint4* const vc = reinterpret_cast<uint4*>(p.v_codes);
+  auto unit = [&](int64_t row, int u) {
+    return u < D / 32 ? kc + row * (D / 32) + u : vc + row * (D / 32) + (u - D / 32);
+  };
+  auto word = [&](int64_t row, int w) {
+    return w < G ? p.k_scale + row * G + w
+                 : (w < 2 * G ? p.v_scale + row * G + (w - G) : reinterpret_cast<uint32_t*>(p.scores) + row);
+  };
+  const int step = cs * kRows;
+  for (int r0 = rank * kRows; r0 - rank * kRows < p.budget; r0 += step) {
+    uint4 x[kUnits];
+    uint32_t y[kWords];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int j = k * kEvThreads + tid, r = r0 + j / kRowUnits;
+      if (r < p.budget) x[k] = *unit(view.row(kept[r]), j % kRowUnits);
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int j = k * kEvThreads + tid, r = r0 + j / kRowWords;
+      if (j < kRows * kRowWords && r < p.budget) y[k] = *word(view.row(kept[r]), j % kRowWords);
+    }
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int j = k * kEvThreads + tid, r = r0 + j / kRowUnits;
+      if (r < p.budget) *unit(view.row(r), j % kRowUnits) = x[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int j = k * kEvThreads + tid, r = r0 + j / kRowWords;
+      if (j < kRows * kRowWords && r < p.budget) *word(view.row(r), j % kRowWords) = y[k];
+    }
+  }
+}
+
+template <int D>
+cudaError_t launch_evict(Kv4EvictParams p, int cs, size_t smem, cudaStream_t s) {
+  static PerDeviceOnce attr;
+  cudaError_t e =
+      attr.run([&] { return cudaFuncSetAttribute(evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.batch * p.kv_heads * cs));
+  cfg.blockDim = dim3(kEvThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = cs;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, evict_kernel<D>, p);
+}
+
+}  // namespace kv4
+}  // namespace afd
+
+using namespace afd;
+
+int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s) {
+  // Small batches spread each (sequence, head) over up to 8 CTAs; two CTAs per SM are the aim.
+  int cs = 1;
+  while (cs < 8 && (int64_t)p.batch * p.kv_heads * cs * 2 <= 2 * device_sm_count()) cs *= 2;
+  const int per = (p.max_blocks * p.block_size + cs - 1) / cs;
+  p.key_cap = per < 200 * 256 ? per : 200 * 256;
+  const size_t smem = (size_t)p.key_cap * 4;
+  switch (dim) {
+    case 64: return (int)kv4::launch_evict<64>(p, cs, smem, s);
+    case 128: return (int)kv4::launch_evict<128>(p, cs, smem, s);
+    default: return (int)kv4::launch_evict<256>(p, cs, smem, s);
+  }
+}

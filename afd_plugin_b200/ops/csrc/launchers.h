@@ -417,3 +417,21 @@ struct Kv4Plan {
 Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len);
 // Returns a cudaError_t.
 int launch_gqa_decode_int4(const Kv4DecodeParams& p, int dtype, cudaStream_t s);
+
+// ---- kv_evict.cu
+struct Kv4EvictParams {
+  uint8_t *k_codes, *v_codes;
+  uint32_t *k_scale, *v_scale;
+  float* scores;              // [blocks, kv_heads, block_size]
+  const int32_t* block_table; // [batch, max_blocks], row stride table_stride
+  const int32_t* seq_lens;
+  int32_t* new_lens;          // [batch]
+  int32_t* kept;              // [batch, kv_heads, budget] positions kept, ascending; -1 past the end
+  int64_t table_stride;
+  int* status;                // or null
+  int batch, kv_heads, block_size, num_blocks, max_blocks;
+  int budget, recent;         // 0 <= recent <= budget, 1 <= budget
+  int key_cap;                // keys a CTA holds in shared memory; set by the launcher
+};
+// Returns a cudaError_t.
+int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s);

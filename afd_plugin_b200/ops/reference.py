@@ -194,8 +194,8 @@ def kv_evict_int4(kv, scores: torch.Tensor, block_table: torch.Tensor, seq_lens:
     hkv, bs = scores.shape[1], scores.shape[2]
     B = seq_lens.shape[0]
     kept = torch.full((B, hkv, budget), -1, dtype=torch.int32, device=scores.device)
-    for b, n in enumerate(seq_lens.tolist()):
-        n = max(n, 0)
+    lens = seq_lens.clamp(0, block_table.shape[1] * bs)
+    for b, n in enumerate(lens.tolist()):
         if n <= budget:
             kept[b, :, :n] = torch.arange(n, dtype=torch.int32, device=scores.device)
             continue
@@ -209,7 +209,7 @@ def kv_evict_int4(kv, scores: torch.Tensor, block_table: torch.Tensor, seq_lens:
             kept[b, h] = keep.int()
             for t in (*kv, scores):
                 t[blk[:budget], h, off[:budget]] = t[blk[keep], h, off[keep]]
-    return seq_lens.clamp(0, budget).to(torch.int32), kept
+    return lens.clamp(max=budget).to(torch.int32), kept
 
 
 # ------------------------------------------------------------- int8 linear

@@ -122,3 +122,37 @@ def test_debug_checks_name_the_bad_entry():
                                 torch.tensor([3], dtype=torch.int32), 1.0)
     finally:
         ops.checks.enable(False)
+
+
+@pytest.mark.parametrize("recent", [0, 3, 8])
+def test_evict_keeps_the_best_and_the_recent(recent):
+    g = torch.Generator().manual_seed(recent)
+    bs, budget, lens = 16, 8, [37, 8, 0, 20]
+    kv = ops.int4_kv_cache(9, bs, 2, 64, device="cpu")
+    for t in (kv.k, kv.v):
+        t.copy_(torch.randint(0, 256, t.shape, generator=g))
+    for t in (kv.k_scale, kv.v_scale):
+        t.copy_(torch.randn(t.shape, generator=g))
+    scores = torch.randint(0, 4, kv.k.shape[:3], generator=g).float()  # ties
+    scores[1, 0, 2], scores[1, 0, 3] = float("nan"), float("inf")
+    table = torch.tensor([[1, 4, 2], [5, 0, 0], [0, 0, 0], [7, 3, 0]], dtype=torch.int32)
+    old = [t.clone() for t in (*kv, scores)]
+    new, kept = ops.kv_evict_int4(kv, scores, table, torch.tensor(lens, dtype=torch.int32), budget, recent)
+    assert new.tolist() == [8, 8, 0, 8]
+    at = lambda b, i: (int(table[b, i // bs]), i % bs)  # noqa: E731
+    for b, n in enumerate(lens):
+        for h in range(2):
+            keep = list(range(n))
+            if n > budget:
+                w = [old[4][at(b, i)[0], h, at(b, i)[1]].item() for i in range(n - recent)]
+                rank = sorted(range(n - recent), key=lambda i: (-(w[i] if w[i] == w[i] else -math.inf), i))
+                keep = sorted(rank[: budget - recent]) + list(range(n - recent, n))
+            assert kept[b, h].tolist() == keep + [-1] * (budget - len(keep))
+            for i in range(n):  # kept rows first, the rest as they were
+                src = at(b, keep[i] if i < len(keep) else i)
+                for t, o in zip((*kv, scores), old):
+                    torch.testing.assert_close(t[at(b, i)[0], h, at(b, i)[1]], o[src[0], h, src[1]], rtol=0, atol=0,
+                                               equal_nan=True)
+    for a in ((0, 0), (4, 5), (4, -1)):
+        with pytest.raises(ValueError):
+            ops.kv_evict_int4(kv, scores, table, torch.tensor(lens, dtype=torch.int32), *a)
