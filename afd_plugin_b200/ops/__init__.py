@@ -419,6 +419,51 @@ def kv_evict_int4(
     return ref.kv_evict_int4(kv, scores, block_table, seq_lens, budget, recent)
 
 
+# ------------------------------------------------------------- int8 linear
+def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of ``x [rows, k]`` as int8 with one fp32 scale each (``x ~ q * scale[:, None]``).
+
+    Tokens are quantised this way inside :func:`int8_linear`; the rows of a weight ``[n, k]`` give
+    its ``w`` and per-channel ``w_scale``.  ``k`` must be a multiple of 16, at most 131072 (the
+    int32 sums cannot overflow).  A row with a value that is not finite gets a scale that is not.
+    """
+    if _cuda(x):
+        return _cuda_ops().int8_quantize(x)
+    _check_int8("int8_quantize", x)
+    return ref.int8_quantize(x)
+
+
+def int8_linear(
+    x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, out_dtype: torch.dtype | None = None
+) -> torch.Tensor:
+    """``x @ (w * w_scale[:, None]).T`` with the tokens quantised to int8 row by row.
+
+    ``x [T, k]`` bf16, fp16 or fp32; ``w [n, k]`` int8 and ``w_scale [n]`` fp32 from
+    :func:`int8_quantize`; the result ``[T, n]`` has ``x``'s type unless ``out_dtype`` names another.
+    The integer sums are exact.
+    """
+    if _cuda(x):
+        return _cuda_ops().int8_linear(x, w, w_scale, out_dtype or x.dtype)
+    _check_int8("int8_linear", x)
+    if w.dtype != torch.int8 or w.dim() != 2 or w.shape[1] != x.shape[1] or not w.shape[0] or not w.is_contiguous():
+        raise ValueError(f"int8_linear: int8 contiguous w [n, {x.shape[1]}], got {tuple(w.shape)} {w.dtype}")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (w.shape[0],):
+        raise ValueError(f"int8_linear: fp32 w_scale [{w.shape[0]}]")
+    if (out_dtype or x.dtype) not in _INT8_IO:
+        raise ValueError("int8_linear: bf16, fp16 or fp32 output")
+    return ref.int8_linear(x, w, w_scale, out_dtype or x.dtype)
+
+
+_INT8_IO = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _check_int8(op: str, x: torch.Tensor) -> None:
+    if x.dim() != 2 or x.dtype not in _INT8_IO:
+        raise ValueError(f"{op}: x [rows, k] in bf16, fp16 or fp32, got {tuple(x.shape)} {x.dtype}")
+    if x.shape[1] % 16 or not 0 < x.shape[1] <= 131072:
+        raise ValueError(f"{op}: k must be a multiple of 16, at most 131072, got {x.shape[1]}")
+
+
 # -------------------------------------------------------------------- MoE
 def moe_experts(
     x: torch.Tensor,
@@ -517,6 +562,8 @@ __all__ = [
     "gqa_decode_int4",
     "head_linear",
     "int4_kv_cache",
+    "int8_linear",
+    "int8_quantize",
     "kv_evict_int4",
     "linear",
     "mla_cache_write",

@@ -710,6 +710,60 @@ std::tuple<at::Tensor, at::Tensor> kv_evict_int4(at::Tensor& kc, at::Tensor& ks,
   return {new_lens, kept};
 }
 
+// ------------------------------------------------------------- int8 linear
+std::tuple<at::Tensor, at::Tensor> int8_quantize(const at::Tensor& x) {
+  const char* op = "int8_quantize";
+  check_cuda(x, "x");
+  TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), op, ": x [rows, k], dense rows");
+  const int64_t t = x.size(0), k = x.size(1);
+  TORCH_CHECK(k > 0 && k % 16 == 0 && k <= 131072, op, ": k must be a multiple of 16, at most 131072, got ",
+              std::to_string(k));
+  TORCH_CHECK(t <= INT32_MAX, op, ": at most 2^31 - 1 rows");
+  const int dt = dtype_code(x);
+  c10::cuda::CUDAGuard g(x.device());
+  auto q = at::empty({t, k}, x.options().dtype(at::kChar));
+  auto scale = at::empty({t}, x.options().dtype(at::kFloat));
+  if (t == 0) return {q, scale};
+  const int64_t per16 = 16 / x.element_size();
+  const bool vec = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) % per16 == 0;
+  C10_CUDA_CHECK((cudaError_t)launch_int8_quantize(q.data_ptr<int8_t>(), scale.data_ptr<float>(), x.data_ptr(),
+                                                   x.stride(0), (int)t, (int)k, vec, dt, stream()));
+  return {q, scale};
+}
+
+at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
+                       at::ScalarType out_dtype) {
+  const char* op = "int8_linear";
+  check_cuda(x, "x");
+  TORCH_CHECK(x.dim() == 2, op, ": x [tokens, k]");
+  check_same_device(w, x, op, "w");
+  check_same_device(w_scale, x, op, "w_scale");
+  TORCH_CHECK(w.scalar_type() == at::kChar && w.dim() == 2 && w.is_contiguous() && w.size(1) == x.size(1) &&
+                  reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0, op,
+              ": int8 contiguous w [n, k], 16-byte aligned, k as in x");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= (1 << 24) && x.size(0) <= (1 << 24), op, ": 1 <= n <= 2^24, tokens <= 2^24");
+  TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.dim() == 1 && w_scale.size(0) == w.size(0) &&
+                  (w.size(0) <= 1 || w_scale.stride(0) == 1), op, ": fp32 w_scale [n]");
+  TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf || out_dtype == at::kFloat, op,
+              ": bf16, fp16 or fp32 output");
+  c10::cuda::CUDAGuard g(x.device());
+  auto [q, s] = int8_quantize(x);
+  auto y = at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
+  if (x.size(0) == 0) return y;
+  Int8GemmParams p{};
+  p.y = y.data_ptr();
+  p.xq = q.data_ptr<int8_t>();
+  p.xs = s.data_ptr<float>();
+  p.w = w.data_ptr<int8_t>();
+  p.ws = w_scale.data_ptr<float>();
+  p.status = status_ptr_or_null(x);
+  p.t = (int)x.size(0);
+  p.n = (int)w.size(0);
+  p.k = (int)x.size(1);
+  C10_CUDA_CHECK((cudaError_t)launch_int8_gemm(p, dtype_code(y), stream()));
+  return y;
+}
+
 // -------------------------------------------------------------------- MoE
 std::vector<at::Tensor> moe_align(const at::Tensor& topk_ids, int64_t e_local, int64_t offset, int64_t n_shared) {
   check_cuda(topk_ids, "topk_ids");
@@ -1434,6 +1488,8 @@ TORCH_LIBRARY(afd_b200, m) {
         "float scale, Tensor(a!)? scores, bool return_lse) -> (Tensor, Tensor)");
   m.def("kv_evict_int4(Tensor(a!) kc, Tensor(b!) ks, Tensor(c!) vc, Tensor(d!) vs, Tensor(e!) scores, "
         "Tensor block_table, Tensor seq_lens, int budget, int recent) -> (Tensor, Tensor)");
+  m.def("int8_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("int8_linear(Tensor x, Tensor w, Tensor w_scale, ScalarType out_dtype) -> Tensor");
   m.def("moe_align(Tensor topk_ids, int e_local, int offset, int n_shared) -> Tensor[]");
   m.def("moe_gather(Tensor x, Tensor row_token, Tensor total) -> Tensor");
   m.def("grouped_gemm(Tensor a, Tensor w, Tensor offsets, Tensor counts, int epilogue) -> Tensor");
@@ -1496,6 +1552,8 @@ TORCH_LIBRARY_IMPL(afd_b200, CUDA, m) {
   m.impl("gqa_cache_write_int4", &gqa_cache_write_int4);
   m.impl("gqa_cache_read_int4", &gqa_cache_read_int4);
   m.impl("gqa_decode_int4", &gqa_decode_int4);
+  m.impl("int8_quantize", &int8_quantize);
+  m.impl("int8_linear", &int8_linear);
   m.impl("kv_evict_int4", &kv_evict_int4);
   m.impl("moe_align", &moe_align);
   m.impl("moe_gather", &moe_gather);

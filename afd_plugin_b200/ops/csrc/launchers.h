@@ -435,3 +435,18 @@ struct Kv4EvictParams {
 };
 // Returns a cudaError_t.
 int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s);
+
+// ---- int8_gemm.cu (both return a cudaError_t)
+// q [t, k] = rows of x (stride ld elements) as int8, scale [t]; k % 8 == 0.
+int launch_int8_quantize(int8_t* q, float* scale, const void* x, int64_t ld, int t, int k, int vec, int dtype,
+                         cudaStream_t s);
+struct Int8GemmParams {
+  void* y;            // [t, n]
+  const int8_t* xq;   // [t, k], k % 16 == 0
+  const float* xs;    // [t]
+  const int8_t* w;    // [n, k]
+  const float* ws;    // [n]
+  int* status;
+  int t, n, k;
+};
+int launch_int8_gemm(const Int8GemmParams& p, int dtype, cudaStream_t s);
