@@ -481,7 +481,8 @@ Kv4Shape check_kv4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor&
   TORCH_CHECK(kc.size(2) > 0 && kc.size(2) % 16 == 0, op, ": block size must be a multiple of 16, got ",
               std::to_string(kc.size(2)));
   TORCH_CHECK(kc.size(0) > 0 && kc.size(1) > 0 && kc.size(0) <= INT32_MAX && kc.size(1) <= 65535 &&
-                  kc.size(2) <= INT32_MAX / 2, op, ": empty or oversized cache");
+                  kc.size(2) <= INT32_MAX / 2 && kc.size(1) * kc.size(2) * d <= INT32_MAX, op,
+              ": empty cache, or blocks of 1 GB and more");
   for (const at::Tensor* t : {&kc, &vc}) {
     TORCH_CHECK(t->scalar_type() == at::kByte && t->sizes() == kc.sizes(), op, ": uint8 codes of one shape");
   }

@@ -31,6 +31,8 @@
 //
 // Scores: a second pass over K alone, with the joined log-sum-exp, adds each
 // position's probability (summed over the group's query heads) to its score.
+#include <type_traits>
+
 #include "device_state.h"
 #include "kv_int4.cuh"
 #include "launchers.h"
@@ -39,28 +41,35 @@ namespace afd {
 namespace kv4 {
 
 constexpr int kTile = 16;
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kStages = 4;
 constexpr int kDecThreads = kWarps * 32;
 constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
+// What a piece costs beside its tiles (pipeline fill, query, merge), in tiles.
+constexpr int kPieceCost = 4;
+constexpr int kMinShare = 8;         // a CTA's share of tiles is not cut below this
 
 template <int D>
 struct Ring {
-  static constexpr int kCodes = kTile * D / 2;          // bytes of one tile's codes
-  static constexpr int kPairs = kTile * (D / kGroup) * 4;
+  static constexpr int G = D / kGroup;
+  static constexpr int kCodes = kTile * D / 2;  // bytes of one tile's codes
+  static constexpr int kPairs = kTile * G * 4;
   static constexpr int kHalf = kCodes + kPairs;  // K codes, K pairs; then the same of V
   static constexpr int kStageBytes = 2 * kHalf;
 };
 
 // 16-byte chunk of a row of codes -> chunk in shared memory.  The MMA operand
 // loads of one instruction touch rows {0, 1, 2, 3}, {4, .., 7} (V) or
-// {0, 4, 1, 5}, {2, 6, 3, 7} (K); this spreads each set over all banks.
+// {0, 4, 1, 5}, {2, 6, 3, 7} (K); this spreads each set over all banks.  Dim
+// group j is reached by an XOR with 32 j, row r + 4 by one with kRow4.
 template <int D>
-AFD_DEVICE int swz(int row, int chunk) {
-  if constexpr (D == 256) return chunk ^ (((row & 3) ^ ((row >> 1) & 2)) << 1);
-  if constexpr (D == 128) return chunk ^ ((((row >> 1) ^ (row >> 2)) & 1) << 1);
+AFD_DEVICE constexpr int swz(int row, int chunk) {
+  if (D == 256) return chunk ^ (((row & 3) ^ ((row >> 1) & 2)) << 1);
+  if (D == 128) return chunk ^ ((((row >> 1) ^ (row >> 2)) & 1) << 1);
   return chunk;
 }
+template <int D> constexpr int kRow4 = D == 256 ? 64 : (D == 128 ? 32 : 0);
 
 template <typename T> struct Codes;  // nibble pairs -> two values c - 8 of T
 template <> struct Codes<__nv_bfloat16> {
@@ -119,6 +128,18 @@ AFD_DEVICE uint32_t lds32(uint32_t addr) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(a) : "r"(addr));
   return a;
 }
+template <int G>
+AFD_DEVICE void lds_pairs(uint32_t (&v)[G], uint32_t addr) {  // one position's (step, zero) pairs
+  if constexpr (G == 1) {
+    v[0] = lds32(addr);
+  } else if constexpr (G == 2) {
+    lds64(v[0], v[1], addr);
+  } else {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(addr));
+  }
+}
 
 // Sequence length as the kernels use it: never negative, never past the table.
 AFD_DEVICE int seq_len_of(const Kv4DecodeParams& p, int b) {
@@ -130,15 +151,19 @@ AFD_DEVICE int seq_len_of(const Kv4DecodeParams& p, int b) {
 // order 0 4 1 5 2 6 3 7 (+ 8), which keeps both operands' loads conflict-free.
 AFD_DEVICE int tile_row(int i) { return (i & 8) | ((i & 7) >> 1) | ((i & 1) << 2); }
 
-// Inclusive prefix sums of the sequences' tile counts into cum[1 .. batch]
+AFD_DEVICE int tiles_of(int n) { return (n + kTile - 1) / kTile; }
+// Length of a (sequence, head chunk) in the order the shares are cut from.
+AFD_DEVICE int cost_of(int tiles) { return tiles > 0 ? tiles + kPieceCost : 0; }
+
+// Inclusive prefix sums of the sequences' costs into cum[1 .. batch]
 // (cum[0] = 0); every thread of the block calls this.
-AFD_DEVICE void tile_prefix(const Kv4DecodeParams& p, int* cum, int* warp_sums) {
+AFD_DEVICE void cost_prefix(const Kv4DecodeParams& p, int* cum, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, nw = blockDim.x / 32;
   int carry = 0;
   if (threadIdx.x == 0) cum[0] = 0;
   for (int b0 = 0; b0 < p.batch; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
-    int v = b < p.batch ? (seq_len_of(p, b) + kTile - 1) / kTile : 0;
+    int v = b < p.batch ? cost_of(tiles_of(seq_len_of(p, b))) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -158,17 +183,21 @@ AFD_DEVICE void tile_prefix(const Kv4DecodeParams& p, int* cum, int* warp_sums) 
   __syncthreads();
 }
 
-// The share of tiles a CTA takes (the same expression wherever it is needed).
-AFD_DEVICE int64_t tiles_per_cta(int64_t total, int ctas) { return (total + ctas - 1) / ctas; }
+// The share of the batch's cost a CTA takes (the same expression wherever it is needed).
+AFD_DEVICE int64_t share_of(int64_t total, int ctas) {
+  const int64_t s = (total + ctas - 1) / ctas;
+  return s < kMinShare + kPieceCost ? kMinShare + kPieceCost : s;
+}
 
 // One piece: tiles [t0, t1) of (sequence b, head chunk hv).
 struct Piece {
-  int b, hv, t0, t1;
-  bool whole;  // covers all tiles of (b, hv)
+  int b, hv, t0, t1, tiles;
+  int64_t next;  // where the next piece starts
 };
 
-// Finds the piece that starts at position `at` of the batch's tile order and
-// ends at `end` or at its (sequence, head)'s last tile.
+// The piece that starts at position `at` of the batch's order and ends at `end`
+// or at its (sequence, head)'s end.  It may hold no tile (t0 == t1), when only
+// a (sequence, head)'s fixed cost fell into the share.
 AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, int64_t end) {
   int lo = 0, hi = batch - 1;  // largest b with cum[b] * heads_v <= at
   while (lo < hi) {
@@ -176,64 +205,92 @@ AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, in
     if ((int64_t)cum[mid] * heads_v <= at) lo = mid;
     else hi = mid - 1;
   }
-  const int tiles = cum[lo + 1] - cum[lo];
+  const int cost = cum[lo + 1] - cum[lo];
   const int64_t rem = at - (int64_t)cum[lo] * heads_v;
   Piece pc;
   pc.b = lo;
-  pc.hv = (int)(rem / tiles);
-  pc.t0 = (int)(rem % tiles);
-  pc.t1 = (int)min((int64_t)tiles, pc.t0 + (end - at));
-  pc.whole = pc.t0 == 0 && pc.t1 == tiles;
+  pc.hv = (int)(rem / cost);
+  const int v0 = (int)(rem - (int64_t)pc.hv * cost);
+  const int v1 = (int)min((int64_t)cost, v0 + (end - at));
+  pc.tiles = cost - kPieceCost;
+  pc.t0 = max(0, v0 - kPieceCost);
+  pc.t1 = max(0, v1 - kPieceCost);
+  pc.next = at + (v1 - v0);
   return pc;
 }
 
-// A warp's view of one (sequence, KV head) in the cache.
+// A warp's walk over the tiles of one (sequence, KV head) in the cache, every
+// kWarps-th tile from `first` on.  Block ids are fetched one tile ahead.
 template <int D>
-struct TileSource {
-  const uint8_t *kc, *vc;
-  const uint8_t *ks, *vs;  // (step, zero) pairs, bytes
+struct TileWalk {
+  const uint8_t *kc, *vc, *sc;  // this lane's bytes of the head's first row: K codes, V codes, pairs
   const int32_t* table;
-  int64_t head_off;        // first position of the head inside a block's rows
-  int64_t block_rows;      // rows (head, position) of one block
-  int block_size, num_blocks;
+  uint32_t block_codes, block_pairs;  // bytes of a block's codes and pairs
+  int pg, in, per_block, step_pg, step_in, num_blocks, blk;
   int* status;
 
-  AFD_DEVICE TileSource(const Kv4DecodeParams& p, int b, int kv_head)
-      : kc(p.k_codes), vc(p.v_codes), ks(reinterpret_cast<const uint8_t*>(p.k_scale)),
-        vs(reinterpret_cast<const uint8_t*>(p.v_scale)), table(p.block_table + (int64_t)b * p.table_stride),
-        head_off((int64_t)kv_head * p.block_size), block_rows((int64_t)p.kv_heads * p.block_size),
-        block_size(p.block_size), num_blocks(p.num_blocks), status(p.status) {}
-
-  // First cache row of tile t.  A block id outside the pool is reported and
-  // replaced by the padding block.
-  AFD_DEVICE int64_t row_of(int t) const {
-    const int pos = t * kTile;
-    const int pg = pos / block_size;
-    int blk = table[pg];
+  AFD_DEVICE TileWalk(const Kv4DecodeParams& p, int b, int kv_head, int first, int lane)
+      : table(p.block_table + (int64_t)b * p.table_stride), num_blocks(p.num_blocks), status(p.status) {
+    const uint32_t rows = (uint32_t)kv_head * p.block_size;
+    kc = p.k_codes + (size_t)rows * (D / 2) + lane * 16;
+    vc = p.v_codes + (size_t)rows * (D / 2) + lane * 16;
+    // the lower half warp copies K's pairs, the upper half V's
+    sc = reinterpret_cast<const uint8_t*>(lane < 16 ? p.k_scale : p.v_scale) + (size_t)rows * (D / kGroup * 4) +
+         (lane & 15) * 16;
+    block_codes = (uint32_t)p.kv_heads * p.block_size * (D / 2);
+    block_pairs = (uint32_t)p.kv_heads * p.block_size * (D / kGroup * 4);
+    per_block = p.block_size / kTile;
+    pg = first / per_block;
+    in = first - pg * per_block;
+    step_pg = kWarps / per_block;
+    step_in = kWarps - step_pg * per_block;
+  }
+  // Reads the block id of the current tile.  One outside the pool is reported
+  // and replaced by the padding block.
+  AFD_DEVICE void fetch() {
+    blk = table[pg];
     if ((unsigned)blk >= (unsigned)num_blocks) {
       if (status != nullptr) atomicExch(status, kStatusBadIndex);
       blk = 0;
     }
-    return blk * block_rows + head_off + (pos - pg * block_size);
   }
-
-  template <bool kWithV>
-  AFD_DEVICE void load(uint32_t stage, int64_t row, int lane) const {
-    using R = Ring<D>;
-    constexpr int kChunks = D / 32;  // 16-byte chunks of a row of codes
-#pragma unroll
-    for (int u = 0; u < kTile * kChunks / 32; ++u) {
-      const int i = u * 32 + lane;
-      const int r = i / kChunks, c = i % kChunks;
-      const uint32_t dst = stage + r * (D / 2) + swz<D>(r, c) * 16;
-      cp16(dst, kc + row * (D / 2) + i * 16);
-      if (kWithV) cp16(dst + R::kHalf, vc + row * (D / 2) + i * 16);
+  AFD_DEVICE void advance() {
+    pg += step_pg;
+    in += step_in;
+    if (in >= per_block) {
+      in -= per_block;
+      ++pg;
     }
-    constexpr int kPairChunks = R::kPairs / 16;  // at most 16: K's by the lower half warp, V's by the upper
-    const int l = lane & 15;
-    if (l < kPairChunks && (kWithV || lane < 16))
-      cp16(stage + (lane < 16 ? 0 : R::kHalf) + R::kCodes + l * 16,
-           (lane < 16 ? ks : vs) + row * (D / kGroup) * 4 + l * 16);
+  }
+  // `dst` / `dst_odd`: this lane's swizzled place in the stage (see lane_places).
+  template <bool kWithV>
+  AFD_DEVICE void load(uint32_t stage, uint32_t dst, int lane) const {
+    using R = Ring<D>;
+    const size_t off = (size_t)blk * block_codes + (uint32_t)(in * R::kCodes);
+#pragma unroll
+    for (int u = 0; u < R::kCodes / 512; ++u) {
+      // 32 chunks on: the row grows by 8 (D = 128) or 4 (D = 256)
+      const uint32_t to = stage + ((D == 256 && (u & 1)) ? dst ^ 64u : dst) + u * 512;
+      cp16(to, kc + off + u * 512);
+      if (kWithV) cp16(to + R::kHalf, vc + off + u * 512);
+    }
+    if ((lane & 15) < R::kPairs / 16 && (kWithV || lane < 16))
+      cp16(stage + R::kCodes + (lane < 16 ? 0 : R::kHalf) + (lane & 15) * 16,
+           sc + (size_t)blk * block_pairs + (uint32_t)(in * R::kPairs));
+  }
+};
+
+// Where this lane copies to and reads from inside a stage.
+template <int D>
+struct Places {
+  uint32_t cp, k, v, pair;
+  AFD_DEVICE explicit Places(int lane) {
+    constexpr int kChunks = D / 32;
+    const int g = lane >> 2, c = lane & 3, r0 = tile_row(g);
+    cp = lane / kChunks * (D / 2) + swz<D>(lane / kChunks, lane % kChunks) * 16;
+    k = r0 * (D / 2) + swz<D>(r0, c >> 1) * 16 + (c & 1) * 8;
+    v = Ring<D>::kHalf + c * (D / 2) + swz<D>(c, g >> 2) * 16 + (g & 3) * 4;
+    pair = Ring<D>::kCodes + r0 * (D / kGroup) * 4;
   }
 };
 
@@ -276,19 +333,18 @@ struct Query {
 // s[t][i] for this lane: rows tile_row(g) (i = 0, 1) and tile_row(g) + 8
 // (i = 2, 3), heads t * 8 + 2c + (i & 1); in the log2 domain.
 template <typename T, int D, int NT>
-AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_t stage, float scale_log2, int lane) {
-  using R = Ring<D>;
+AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
+                            float scale_log2) {
   constexpr int G = D / kGroup;
-  const int c = lane & 3, r0 = tile_row(lane >> 2);
-  const uint32_t pairs = stage + R::kCodes;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+  uint32_t p0[G], p1[G];
+  lds_pairs<G>(p0, stage + at.pair);
+  lds_pairs<G>(p1, stage + at.pair + 8 * G * 4);
 #pragma unroll
   for (int j = 0; j < G; ++j) {
     uint32_t w0[2], w1[2];
-    const int chunk = 2 * j + (c >> 1);
-    lds64(w0[0], w0[1], stage + r0 * (D / 2) + swz<D>(r0, chunk) * 16 + (c & 1) * 8);
-    lds64(w1[0], w1[1], stage + (r0 + 8) * (D / 2) + swz<D>(r0 + 8, chunk) * 16 + (c & 1) * 8);
+    const uint32_t from = (stage + at.k) ^ (j * 32);
+    lds64(w0[0], w0[1], from);
+    lds64(w1[0], w1[1], from + 8 * (D / 2));
     float acc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
@@ -300,16 +356,22 @@ AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_
 #pragma unroll
       for (int t = 0; t < NT; ++t) mma<T>(acc[t], a0, a1, a2, a3, q.f[t][j * 4 + k][0], q.f[t][j * 4 + k][1]);
     }
-    const uint32_t p0 = lds32(pairs + (r0 * G + j) * 4), p1 = lds32(pairs + ((r0 + 8) * G + j) * 4);
-    const float st0 = pair_step(p0), st1 = pair_step(p1);
-    const float z0 = fmaf(8.f, st0, pair_zero(p0)), z1 = fmaf(8.f, st1, pair_zero(p1));
+    const float st0 = pair_step(p0[j]), st1 = pair_step(p1[j]);
+    const float z0 = fmaf(8.f, st0, pair_zero(p0[j])), z1 = fmaf(8.f, st1, pair_zero(p1[j]));
     const float m0 = st0 * scale_log2, m1 = st1 * scale_log2;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      s[t][0] += fmaf(m0, acc[t][0], z0 * q.sum[t][j][0]);
-      s[t][1] += fmaf(m0, acc[t][1], z0 * q.sum[t][j][1]);
-      s[t][2] += fmaf(m1, acc[t][2], z1 * q.sum[t][j][0]);
-      s[t][3] += fmaf(m1, acc[t][3], z1 * q.sum[t][j][1]);
+      if (j == 0) {
+        s[t][0] = fmaf(m0, acc[t][0], z0 * q.sum[t][j][0]);
+        s[t][1] = fmaf(m0, acc[t][1], z0 * q.sum[t][j][1]);
+        s[t][2] = fmaf(m1, acc[t][2], z1 * q.sum[t][j][0]);
+        s[t][3] = fmaf(m1, acc[t][3], z1 * q.sum[t][j][1]);
+      } else {
+        s[t][0] = fmaf(m0, acc[t][0], fmaf(z0, q.sum[t][j][0], s[t][0]));
+        s[t][1] = fmaf(m0, acc[t][1], fmaf(z0, q.sum[t][j][1], s[t][1]));
+        s[t][2] = fmaf(m1, acc[t][2], fmaf(z1, q.sum[t][j][0], s[t][2]));
+        s[t][3] = fmaf(m1, acc[t][3], fmaf(z1, q.sum[t][j][1], s[t][3]));
+      }
     }
   }
 }
@@ -363,70 +425,12 @@ AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int hea
   }
 }
 
-template <typename T, int D, int NT, int kStages>
-__global__ void __launch_bounds__(kDecThreads, (D * NT <= 128 ? 2 : 1)) decode_kernel(Kv4DecodeParams p) {
-  using R = Ring<D>;
-  constexpr int G = D / kGroup, H = NT * 8;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int s_warp[kWarps];
-  __shared__ float s_ml[2 * kWarps * H];
-  uint8_t* ring = smem;  // reused by the warps' results once a piece is done
-  T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
-  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c = lane & 3;
-  const int heads_v = p.kv_heads * p.chunks;
-
-  int64_t at, end;
-  if (p.direct) {
-    at = 0;  // one (sequence, head chunk) per CTA
-    end = 1;
-  } else {
-    tile_prefix(p, cum, s_warp);
-    const int64_t total = (int64_t)cum[p.batch] * heads_v;
-    const int64_t per = tiles_per_cta(total, gridDim.x);
-    at = min(total, blockIdx.x * per);
-    end = min(total, at + per);
-  }
-  const int64_t first = at;
-  while (at < end) {
-    Piece pc;
-    if (p.direct) {
-      pc.b = blockIdx.x / heads_v;
-      pc.hv = blockIdx.x % heads_v;
-      pc.t0 = 0;
-      pc.t1 = (seq_len_of(p, pc.b) + kTile - 1) / kTile;
-      pc.whole = true;
-      at = end;
-    } else {
-      pc = piece_at(cum, p.batch, heads_v, at, end);
-    }
-    const int n = seq_len_of(p, pc.b);
-    const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
-    const int h_in = pc.hv % p.chunks * H;
-    const int heads = min(H, group - h_in);
-    const int head0 = kv_head * group + h_in;
-    const TileSource<D> src(p, pc.b, kv_head);
-    const uint32_t base = smem_u32(ring) + warp * kStages * R::kStageBytes;
-
-    // Fill the ring.  Tiles of a piece are dealt to the warps in turn.
-    int issue = pc.t0 + warp;
-    int64_t row = issue < pc.t1 ? src.row_of(issue) : 0;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      if (issue < pc.t1) {
-        src.template load<true>(base + s * R::kStageBytes, row, lane);
-        issue += kWarps;
-        if (issue < pc.t1) row = src.row_of(issue);
-      }
-      cp_commit();
-    }
-    stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
-    __syncthreads();
-    Query<T, D, NT> q;
-    q.load(sq, p.scale_log2, lane);
-
-    float o[NT][G * 4][4], zo[NT][G][2], m[NT][2], l[NT][2];
+// The running state of one warp: its 8 NT heads' maxima and sums, and o.
+template <int D, int NT>
+struct Acc {
+  static constexpr int G = D / kGroup;
+  float o[NT][G * 4][4], zo[NT][G][2], m[NT][2], l[NT][2];
+  AFD_DEVICE void clear() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -436,114 +440,201 @@ __global__ void __launch_bounds__(kDecThreads, (D * NT <= 128 ? 2 : 1)) decode_k
       m[t][0] = m[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
+  }
+};
 
-    int stage = 0;
-    const int r0 = tile_row(g);
+// One tile in a stage of the ring.  `left` positions of it exist (kTail: fewer
+// than 16): the others weigh nothing, whatever their bytes hold.
+template <typename T, int D, int NT, bool kTail>
+AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
+                          float scale_log2, int left, int lane) {
+  using R = Ring<D>;
+  constexpr int G = D / kGroup;
+  // bf16 results take p * step rounded to bf16; fp16 ones take a second,
+  // low part as well, so that the output's own rounding stays the larger.
+  constexpr int kParts = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
+  float s[NT][4];
+  tile_logits<T, D, NT>(s, q, stage, at, scale_log2);
+  const int r0 = tile_row(lane >> 2);
+  const bool in0 = !kTail || r0 < left, in1 = !kTail || r0 + 8 < left;
+  bool grow = false;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (!in0) s[t][0] = s[t][1] = -INFINITY;
+    if (!in1) s[t][2] = s[t][3] = -INFINITY;
+    grow |= fmaxf(s[t][0], s[t][2]) > acc.m[t][0] + kLazy || fmaxf(s[t][1], s[t][3]) > acc.m[t][1] + kLazy;
+  }
+  if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[t][e], s[t][2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(mx, acc.m[t][e]);
+        const float f = mx == -INFINITY ? 1.f : fast_exp2(acc.m[t][e] - mx);
+        acc.m[t][e] = mx;
+        acc.l[t][e] *= f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) acc.zo[t][j][e] *= f;
+#pragma unroll
+        for (int i = 0; i < G * 4; ++i) {
+          acc.o[t][i][e] *= f;
+          acc.o[t][i][2 + e] *= f;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // a maximum of -inf is left only where every logit so far is -inf or NaN
+      s[t][i] = fast_exp2(s[t][i] - (acc.m[t][i & 1] == -INFINITY ? 0.f : acc.m[t][i & 1]));
+      acc.l[t][i & 1] += s[t][i];
+    }
+  }
+  // P V: the probabilities, scaled per dim group, are the B operand.
+  uint32_t p0[G], p1[G];
+  lds_pairs<G>(p0, stage + R::kHalf + at.pair);
+  lds_pairs<G>(p1, stage + R::kHalf + at.pair + 8 * G * 4);
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    // positions past the end hold anything: their factors are zero, not 0 * that
+    const float st0 = in0 ? pair_step(p0[j]) : 0.f, st1 = in1 ? pair_step(p1[j]) : 0.f;
+    const float z0 = in0 ? fmaf(8.f, st0, pair_zero(p0[j])) : 0.f, z1 = in1 ? fmaf(8.f, st1, pair_zero(p1[j])) : 0.f;
+    uint32_t b[NT][kParts][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      acc.zo[t][j][0] = fmaf(s[t][0], z0, fmaf(s[t][2], z1, acc.zo[t][j][0]));
+      acc.zo[t][j][1] = fmaf(s[t][1], z0, fmaf(s[t][3], z1, acc.zo[t][j][1]));
+      const float x[4] = {s[t][0] * st0, s[t][1] * st0, s[t][2] * st1, s[t][3] * st1};
+      const uint32_t h0 = pack_bf16(x[0], x[1]), h1 = pack_bf16(x[2], x[3]);
+      b[t][0][0] = transpose8(h0);
+      b[t][0][1] = transpose8(h1);
+      if constexpr (kParts == 2) {
+        b[t][1][0] = transpose8(pack_bf16(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xFFFF0000u)));
+        b[t][1][1] = transpose8(pack_bf16(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xFFFF0000u)));
+      }
+    }
+    // k indices 2c, 2c + 1, 2c + 8, 2c + 9 are rows c, c + 4, c + 8, c + 12
+    const uint32_t even = (stage + at.v) ^ (j * 32), odd = (even ^ kRow4<D>) + 4 * (D / 2);
+    const uint32_t w0 = lds32(even), w1 = lds32(odd), w2 = lds32(even + 8 * (D / 2)), w3 = lds32(odd + 8 * (D / 2));
+    const uint32_t x0 = __byte_perm(w0, w1, 0x5410), x1 = __byte_perm(w0, w1, 0x7632);
+    const uint32_t x2 = __byte_perm(w2, w3, 0x5410), x3 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a0 = Codes<__nv_bfloat16>::pair(x0 >> (4 * i)), a1 = Codes<__nv_bfloat16>::pair(x1 >> (4 * i));
+      const uint32_t a2 = Codes<__nv_bfloat16>::pair(x2 >> (4 * i)), a3 = Codes<__nv_bfloat16>::pair(x3 >> (4 * i));
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < kParts; ++u)
+          mma<__nv_bfloat16>(acc.o[t][j * 4 + i], a0, a1, a2, a3, b[t][u][0], b[t][u][1]);
+    }
+  }
+}
+
+// CTAs of kWarps warps that one SM holds (registers bound it).
+template <int D, int NT> constexpr int kResident = D * NT <= 128 ? 4 : 2;
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel(Kv4DecodeParams p) {
+  using R = Ring<D>;
+  constexpr int G = D / kGroup, H = NT * 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int s_warp[kWarps];
+  __shared__ float s_ml[2 * kWarps * H];
+  T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
+  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int heads_v = p.kv_heads * p.chunks;
+  const Places<D> place(lane);
+
+  int64_t at = 0, end = 1;  // direct: one (sequence, head chunk) per CTA
+  if (!p.direct) {
+    cost_prefix(p, cum, s_warp);
+    const int64_t total = (int64_t)cum[p.batch] * heads_v;
+    const int64_t share = share_of(total, gridDim.x);
+    at = min(total, blockIdx.x * share);
+    end = min(total, at + share);
+  }
+  while (at < end) {
+    Piece pc;
+    if (p.direct) {
+      pc.b = blockIdx.x / heads_v;
+      pc.hv = blockIdx.x % heads_v;
+      pc.t0 = 0;
+      pc.t1 = pc.tiles = tiles_of(seq_len_of(p, pc.b));
+      pc.next = end;
+    } else {
+      pc = piece_at(cum, p.batch, heads_v, at, end);
+      if (pc.t0 == pc.t1) {
+        at = pc.next;
+        continue;
+      }
+    }
+    at = pc.next;
+    const int n = seq_len_of(p, pc.b);
+    const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
+    const int h_in = pc.hv % p.chunks * H;
+    const int heads = min(H, group - h_in);
+    const int head0 = kv_head * group + h_in;
+    const uint32_t base = smem_u32(smem) + warp * kStages * R::kStageBytes;
+
+    // Fill the ring.  Tiles of a piece are dealt to the warps in turn.
+    int issue = pc.t0 + warp;
+    TileWalk<D> walk(p, pc.b, kv_head, issue, lane);
+    if (issue < pc.t1) walk.fetch();
+    auto copy_next = [&](uint32_t into) {
+      if (issue < pc.t1) {
+        walk.template load<true>(into, place.cp, lane);
+        issue += kWarps;
+        walk.advance();
+        if (issue < pc.t1) walk.fetch();
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * R::kStageBytes);
+    stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
+    __syncthreads();
+    Query<T, D, NT> q;
+    q.load(sq, p.scale_log2, lane);
+
+    Acc<D, NT> acc;
+    acc.clear();
+    constexpr uint32_t kLast = (kStages - 1) * R::kStageBytes;
+    uint32_t st = base, into = base + kLast;
     for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
       cp_wait<kStages - 2>();
       __syncwarp();
-      {  // refill the stage that the previous tile has left
-        const int into = stage == 0 ? kStages - 1 : stage - 1;
-        if (issue < pc.t1) {
-          src.template load<true>(base + into * R::kStageBytes, row, lane);
-          issue += kWarps;
-          if (issue < pc.t1) row = src.row_of(issue);
-        }
-        cp_commit();
-      }
-      const uint32_t st = base + stage * R::kStageBytes;
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-
-      float s[NT][4];
-      tile_logits<T, D, NT>(s, q, st, p.scale_log2, lane);
-      const bool in0 = tile * kTile + r0 < n, in1 = tile * kTile + r0 + 8 < n;
-      bool grow = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (!in0) s[t][0] = s[t][1] = -INFINITY;
-        if (!in1) s[t][2] = s[t][3] = -INFINITY;
-        grow |= fmaxf(s[t][0], s[t][2]) > m[t][0] + kLazy || fmaxf(s[t][1], s[t][3]) > m[t][1] + kLazy;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[t][e], s[t][2 + e]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            mx = fmaxf(mx, m[t][e]);
-            const float f = mx == -INFINITY ? 1.f : fast_exp2(m[t][e] - mx);
-            m[t][e] = mx;
-            l[t][e] *= f;
-#pragma unroll
-            for (int j = 0; j < G; ++j) zo[t][j][e] *= f;
-#pragma unroll
-            for (int i = 0; i < G * 4; ++i) {
-              o[t][i][e] *= f;
-              o[t][i][2 + e] *= f;
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float mm = m[t][i & 1];
-          s[t][i] = fast_exp2(s[t][i] - (mm == -INFINITY ? 0.f : mm));
-          l[t][i & 1] += s[t][i];
-        }
-      }
-      // P V: the probabilities, scaled per dim group, are the B operand.
-      const uint32_t pairs = st + R::kHalf + R::kCodes;
-      const uint32_t vbase = st + R::kHalf + (g & 3) * 4;
-#pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const uint32_t p0 = lds32(pairs + (r0 * G + j) * 4), p1 = lds32(pairs + ((r0 + 8) * G + j) * 4);
-        // positions past the end hold anything: their factors are zero, not 0 * that
-        const float st0 = in0 ? pair_step(p0) : 0.f, st1 = in1 ? pair_step(p1) : 0.f;
-        const float z0 = in0 ? fmaf(8.f, st0, pair_zero(p0)) : 0.f, z1 = in1 ? fmaf(8.f, st1, pair_zero(p1)) : 0.f;
-        uint32_t b[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          zo[t][j][0] = fmaf(s[t][0], z0, fmaf(s[t][2], z1, zo[t][j][0]));
-          zo[t][j][1] = fmaf(s[t][1], z0, fmaf(s[t][3], z1, zo[t][j][1]));
-          b[t][0] = transpose8(pack_bf16(s[t][0] * st0, s[t][1] * st0));
-          b[t][1] = transpose8(pack_bf16(s[t][2] * st1, s[t][3] * st1));
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // k indices 2c, 2c + 1, 2c + 8, 2c + 9
-          const int r = tile_row(2 * c + (i & 1)) + (i >> 1) * 8;
-          w[i] = lds32(vbase + r * (D / 2) + swz<D>(r, 2 * j + (g >> 2)) * 16);
-        }
-        const uint32_t a = __byte_perm(w[0], w[1], 0x5410), bb = __byte_perm(w[0], w[1], 0x7632);
-        const uint32_t cc = __byte_perm(w[2], w[3], 0x5410), dd = __byte_perm(w[2], w[3], 0x7632);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t a0 = Codes<__nv_bfloat16>::pair(a >> (4 * i)), a1 = Codes<__nv_bfloat16>::pair(bb >> (4 * i));
-          const uint32_t a2 = Codes<__nv_bfloat16>::pair(cc >> (4 * i)), a3 = Codes<__nv_bfloat16>::pair(dd >> (4 * i));
-#pragma unroll
-          for (int t = 0; t < NT; ++t) mma<__nv_bfloat16>(o[t][j * 4 + i], a0, a1, a2, a3, b[t][0], b[t][1]);
-        }
-      }
+      copy_next(into);  // into the stage that the previous tile has left
+      const int left = n - tile * kTile;
+      if (left >= kTile)
+        take_tile<T, D, NT, false>(acc, q, st, place, p.scale_log2, left, lane);
+      else
+        take_tile<T, D, NT, true>(acc, q, st, place, p.scale_log2, left, lane);
+      into = st;
+      st = st == base + kLast ? base : st + R::kStageBytes;
       __syncwarp();  // every lane is done with this stage before it is refilled
     }
     cp_wait<0>();
     __syncthreads();  // the ring is free: it takes the warps' results
 
     const int nact = min(kWarps, pc.t1 - pc.t0);
-    float* red = reinterpret_cast<float*>(ring);
+    float* red = reinterpret_cast<float*>(smem);
     if (warp < nact) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float ls = l[t][e], z[G];
+          float ls = acc.l[t][e], z[G];
 #pragma unroll
-          for (int j = 0; j < G; ++j) z[j] = zo[t][j][e];
+          for (int j = 0; j < G; ++j) z[j] = acc.zo[t][j][e];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             ls += __shfl_xor_sync(0xffffffffu, ls, x);
@@ -552,28 +643,28 @@ __global__ void __launch_bounds__(kDecThreads, (D * NT <= 128 ? 2 : 1)) decode_k
           }
           const int h = t * 8 + 2 * c + e;
           if (g == 0) {
-            s_ml[warp * H + h] = m[t][e];
+            s_ml[warp * H + h] = acc.m[t][e];
             s_ml[(kWarps + warp) * H + h] = ls;
           }
           float* to = red + ((size_t)warp * H + h) * D + g * 8;
 #pragma unroll
           for (int j = 0; j < G; ++j) {
-            *reinterpret_cast<float4*>(to + j * kGroup) =
-                make_float4(o[t][j * 4][e] + z[j], o[t][j * 4 + 1][e] + z[j], o[t][j * 4 + 2][e] + z[j],
-                            o[t][j * 4 + 3][e] + z[j]);
+            const auto& o = acc.o[t];
+            *reinterpret_cast<float4*>(to + j * kGroup) = make_float4(
+                o[j * 4][e] + z[j], o[j * 4 + 1][e] + z[j], o[j * 4 + 2][e] + z[j], o[j * 4 + 3][e] + z[j]);
             *reinterpret_cast<float4*>(to + j * kGroup + 4) =
-                make_float4(o[t][j * 4][2 + e] + z[j], o[t][j * 4 + 1][2 + e] + z[j], o[t][j * 4 + 2][2 + e] + z[j],
-                            o[t][j * 4 + 3][2 + e] + z[j]);
+                make_float4(o[j * 4][2 + e] + z[j], o[j * 4 + 1][2 + e] + z[j], o[j * 4 + 2][2 + e] + z[j],
+                            o[j * 4 + 3][2 + e] + z[j]);
           }
         }
       }
     }
     __syncthreads();
-    // A CTA's first piece starts its share, its last ends it: two partial slots each.
-    write_result<T, D, NT>(p, pc.b, head0, heads, 2 * (int64_t)blockIdx.x + (at == first ? 0 : 1), pc.whole, red, s_ml,
-                           nact);
+    // Only a share's first and last pieces can be parts of a (sequence, head):
+    // one that begins with its first tile goes to the CTA's second slot.
+    write_result<T, D, NT>(p, pc.b, head0, heads, 2 * (int64_t)blockIdx.x + (pc.t0 == 0 ? 1 : 0),
+                           pc.t0 == 0 && pc.t1 == pc.tiles, red, s_ml, nact);
     __syncthreads();
-    if (!p.direct) at += pc.t1 - pc.t0;
   }
 }
 
@@ -585,7 +676,7 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
   const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   int before = 0, all = 0;
   for (int i = threadIdx.x; i < p.batch; i += blockDim.x) {
-    const int t = (seq_len_of(p, i) + kTile - 1) / kTile;
+    const int t = cost_of(tiles_of(seq_len_of(p, i)));
     all += t;
     if (i < b) before += t;
   }
@@ -601,7 +692,7 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
   __syncthreads();
   before = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
   all = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
-  const int tiles = (seq_len_of(p, b) + kTile - 1) / kTile;
+  const int tiles = tiles_of(seq_len_of(p, b));
   T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head) * dim;
   pdl_wait();
   if (tiles == 0) {
@@ -612,11 +703,11 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
   const int group = p.heads / p.kv_heads;
   const int kv_head = head / group, hc = head % group / heads_chunk, h = head % group % heads_chunk;
   const int heads_v = p.kv_heads * p.chunks;
-  const int64_t per = tiles_per_cta((int64_t)all * heads_v, ctas);
-  const int64_t start = (int64_t)before * heads_v + (int64_t)(kv_head * p.chunks + hc) * tiles;
-  const int64_t c0 = start / per, c1 = (start + tiles - 1) / per;
+  const int64_t share = share_of((int64_t)all * heads_v, ctas);
+  const int64_t start = (int64_t)before * heads_v + (int64_t)(kv_head * p.chunks + hc) * cost_of(tiles) + kPieceCost;
+  const int64_t c0 = start / share, c1 = (start + tiles - 1) / share;
   if (c0 == c1) return;  // one CTA had all of it and wrote the result
-  auto slot = [&](int64_t c) { return (2 * c + (c == c0 && start != c0 * per ? 1 : 0)) * heads_chunk + h; };
+  auto slot = [&](int64_t c) { return (2 * c + (c == c0 ? 1 : 0)) * heads_chunk + h; };
   float m = -INFINITY;
   for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, p.part_ml[slot(c) * 2]);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
@@ -637,48 +728,53 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
 
 // Adds every position's probability to its score.  The same shares of tiles;
 // nothing to merge, since a position is in one tile.
-template <typename T, int D, int NT, int kStages>
-__global__ void __launch_bounds__(kDecThreads, 2) score_kernel(Kv4DecodeParams p) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p) {
   using R = Ring<D>;
   constexpr int H = NT * 8;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_warp[kWarps];
   T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
   int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int c = lane & 3;
+  const int c = lane & 3, r0 = tile_row(lane >> 2);
   const int heads_v = p.kv_heads * p.chunks;
-  tile_prefix(p, cum, s_warp);
+  const Places<D> place(lane);
+  cost_prefix(p, cum, s_warp);
   const int64_t total = (int64_t)cum[p.batch] * heads_v;
-  const int64_t per = tiles_per_cta(total, gridDim.x);
-  int64_t at = min(total, blockIdx.x * per);
-  const int64_t end = min(total, at + per);
+  const int64_t share = share_of(total, gridDim.x);
+  int64_t at = min(total, blockIdx.x * share);
+  const int64_t end = min(total, at + share);
   pdl_wait();  // the log-sum-exps of the decode
   while (at < end) {
     const Piece pc = piece_at(cum, p.batch, heads_v, at, end);
+    at = pc.next;
+    if (pc.t0 == pc.t1) continue;
     const int n = seq_len_of(p, pc.b);
     const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
     const int h_in = pc.hv % p.chunks * H;
     const int heads = min(H, group - h_in);
     const int head0 = kv_head * group + h_in;
-    const TileSource<D> src(p, pc.b, kv_head);
     const uint32_t base = smem_u32(smem) + warp * kStages * R::kHalf;
     int issue = pc.t0 + warp;
-    int64_t row = issue < pc.t1 ? src.row_of(issue) : 0;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
+    TileWalk<D> walk(p, pc.b, kv_head, issue, lane);
+    if (issue < pc.t1) walk.fetch();
+    auto copy_next = [&](uint32_t into) {
       if (issue < pc.t1) {
-        src.template load<false>(base + s * R::kHalf, row, lane);
+        walk.template load<false>(into, place.cp, lane);
         issue += kWarps;
-        if (issue < pc.t1) row = src.row_of(issue);
+        walk.advance();
+        if (issue < pc.t1) walk.fetch();
       }
       cp_commit();
-    }
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * R::kHalf);
     stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
     __syncthreads();
     Query<T, D, NT> q;
     q.load(sq, p.scale_log2, lane);
-    float lse[NT][2];  // log2 domain; heads beyond the group and empty rows weigh nothing
+    float lse[NT][2];  // log2 domain; heads beyond the group weigh nothing
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -686,23 +782,20 @@ __global__ void __launch_bounds__(kDecThreads, 2) score_kernel(Kv4DecodeParams p
         const int h = t * 8 + 2 * c + e;
         lse[t][e] = h < heads ? p.lse[(int64_t)pc.b * p.heads + head0 + h] * 1.4426950408889634f : INFINITY;
       }
-    int stage = 0;
-    const int r0 = tile_row(lane >> 2);
+    // a second walk, for the scores' addresses
+    TileWalk<D> to(p, pc.b, kv_head, pc.t0 + warp, lane);
+    float* const scores = p.scores + (size_t)kv_head * p.block_size;
+    constexpr uint32_t kLast = (kStages - 1) * R::kHalf;
+    uint32_t st = base, into = base + kLast;
     for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
+      to.fetch();
       cp_wait<kStages - 2>();
       __syncwarp();
-      {
-        const int into = stage == 0 ? kStages - 1 : stage - 1;
-        if (issue < pc.t1) {
-          src.template load<false>(base + into * R::kHalf, row, lane);
-          issue += kWarps;
-          if (issue < pc.t1) row = src.row_of(issue);
-        }
-        cp_commit();
-      }
+      copy_next(into);
       float s[NT][4];
-      tile_logits<T, D, NT>(s, q, base + stage * R::kHalf, p.scale_log2, lane);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      tile_logits<T, D, NT>(s, q, st, place, p.scale_log2);
+      into = st;
+      st = st == base + kLast ? base : st + R::kHalf;
       float w0 = 0.f, w1 = 0.f;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -716,29 +809,31 @@ __global__ void __launch_bounds__(kDecThreads, 2) score_kernel(Kv4DecodeParams p
       // Adds, not stores: head chunks and sequences that share blocks meet here.
       if (c < 2) {
         const int r = r0 + c * 8;
-        if (tile * kTile + r < n) atomicAdd(p.scores + src.row_of(tile) + r, c == 0 ? w0 : w1);
+        if (tile * kTile + r < n)
+          atomicAdd(scores + (size_t)to.blk * ((uint32_t)p.kv_heads * p.block_size) + to.in * kTile + r,
+                    c == 0 ? w0 : w1);
       }
+      to.advance();
       __syncwarp();
     }
     cp_wait<0>();
     __syncthreads();
-    at += pc.t1 - pc.t0;
   }
 }
 
-template <typename T, int D, int NT, int kStages>
+template <typename T, int D, int NT>
 cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
   constexpr int H = NT * 8;
-  const int ring = kWarps * kStages * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
+  constexpr int ring = kWarps * kStages * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
   p.ring_bytes = ring > red ? ring : red;
   const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.direct ? 0 : (p.batch + 1) * 4);
   static PerDeviceOnce attr;
   cudaError_t e = attr.run([&] {
-    return cudaFuncSetAttribute(decode_kernel<T, D, NT, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(decode_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
   });
   if (e != cudaSuccess) return e;
-  decode_kernel<T, D, NT, kStages><<<p.ctas, kDecThreads, smem, s>>>(p);
+  decode_kernel<T, D, NT><<<p.ctas, kDecThreads, smem, s>>>(p);
   if (!p.direct) {
     e = launch_pdl(join_kernel<T>, dim3((unsigned)(p.batch * p.heads)), dim3(128), 0, s, p, D, H, p.ctas);
     if (e != cudaSuccess) return e;
@@ -748,22 +843,21 @@ cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
 
 template <typename T, int D, int NT>
 cudaError_t launch_score(Kv4DecodeParams p, cudaStream_t s) {
-  constexpr int kStages = 4, H = NT * 8;
+  constexpr int H = NT * 8;
   p.ring_bytes = kWarps * kStages * Ring<D>::kHalf;
   const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.batch + 1) * 4;
   static PerDeviceOnce attr;
   cudaError_t e = attr.run([&] {
-    return cudaFuncSetAttribute(score_kernel<T, D, NT, kStages>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(score_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
   });
   if (e != cudaSuccess) return e;
-  return launch_pdl(score_kernel<T, D, NT, kStages>, dim3(2 * device_sm_count()), dim3(kDecThreads), (size_t)smem, s,
-                    p);
+  return launch_pdl(score_kernel<T, D, NT>, dim3(4 * device_sm_count()), dim3(kDecThreads), (size_t)smem, s, p);
 }
 
 template <typename T, int D, int NT>
 cudaError_t run(const Kv4DecodeParams& p, cudaStream_t s) {
-  const cudaError_t e = launch_decode<T, D, NT, 4>(p, s);
+  const cudaError_t e = launch_decode<T, D, NT>(p, s);
   if (e != cudaSuccess || p.scores == nullptr) return e;
   return launch_score<T, D, NT>(p, s);
 }
@@ -794,7 +888,7 @@ Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len
   const int64_t items = (int64_t)batch * kv_heads * plan.chunks;
   constexpr int kDirectTiles = 32;
   plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
-  const int resident = dim * plan.head_tiles <= 128 ? 2 : 1;
+  const int resident = dim * plan.head_tiles <= 128 ? 4 : 2;  // kResident
   plan.ctas = plan.direct ? (int)items : resident * device_sm_count();
   plan.max_batch = kv4::kMaxBatch;
   return plan;
