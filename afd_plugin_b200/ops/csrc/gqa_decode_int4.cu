@@ -31,6 +31,7 @@
 //
 // Scores: a second pass over K alone, with the joined log-sum-exp, adds each
 // position's probability (summed over the group's query heads) to its score.
+#include <cfloat>
 #include <type_traits>
 
 #include "device_state.h"
@@ -45,6 +46,7 @@ constexpr int kWarps = 4;
 constexpr int kStages = 4;
 constexpr int kDecThreads = kWarps * 32;
 constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
+constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
 // What a piece costs beside its tiles (pipeline fill, query, merge), in tiles.
 constexpr int kPieceCost = 4;
@@ -71,22 +73,29 @@ AFD_DEVICE constexpr int swz(int row, int chunk) {
 }
 template <int D> constexpr int kRow4 = D == 256 ? 64 : (D == 128 ? 32 : 0);
 
-template <typename T> struct Codes;  // nibble pairs -> two values c - 8 of T
+// Nibbles 0 and 4 of w as two values c - 8 of T.  OR-ing a code into the
+// mantissa of 128 (bf16) or 1024 (fp16) adds it; the subtraction is exact.
+// Mask and base come from the kernel's parameters: as literals they would cost
+// two logic operations instead of one (an instruction takes one literal).
+template <typename T> struct Codes;
 template <> struct Codes<__nv_bfloat16> {
-  // 0x4300 | c is 128 + c in bf16; minus 136 is exact.
-  static AFD_DEVICE uint32_t pair(uint32_t w) {
-    const uint32_t m = (w & 0x000F000Fu) | 0x43004300u;
+  static constexpr uint32_t kBase = 0x43004300u;
+  static AFD_DEVICE uint32_t pair(uint32_t w, uint32_t mask, uint32_t base) {
+    const uint32_t m = (w & mask) | base;
     __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), __floats2bfloat162_rn(136.f, 136.f));
     return *reinterpret_cast<uint32_t*>(&v);
   }
 };
 template <> struct Codes<__half> {
-  // 0x6400 | c is 1024 + c in fp16; minus 1032 is exact.
-  static AFD_DEVICE uint32_t pair(uint32_t w) {
-    const uint32_t m = (w & 0x000F000Fu) | 0x64006400u;
+  static constexpr uint32_t kBase = 0x64006400u;
+  static AFD_DEVICE uint32_t pair(uint32_t w, uint32_t mask, uint32_t base) {
+    const uint32_t m = (w & mask) | base;
     __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1032.f, 1032.f));
     return *reinterpret_cast<uint32_t*>(&v);
   }
+};
+struct Nibbles {
+  uint32_t mask, base_k, base_v;
 };
 
 template <typename T> AFD_DEVICE void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -334,7 +343,7 @@ struct Query {
 // (i = 2, 3), heads t * 8 + 2c + (i & 1); in the log2 domain.
 template <typename T, int D, int NT>
 AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                            float scale_log2) {
+                            float scale_log2, const Nibbles& nb) {
   constexpr int G = D / kGroup;
   uint32_t p0[G], p1[G];
   lds_pairs<G>(p0, stage + at.pair);
@@ -351,8 +360,8 @@ AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t x = w0[k >> 1] >> ((k & 1) * 8), y = w1[k >> 1] >> ((k & 1) * 8);
-      const uint32_t a0 = Codes<T>::pair(x), a2 = Codes<T>::pair(x >> 4);
-      const uint32_t a1 = Codes<T>::pair(y), a3 = Codes<T>::pair(y >> 4);
+      const uint32_t a0 = Codes<T>::pair(x, nb.mask, nb.base_k), a2 = Codes<T>::pair(x >> 4, nb.mask, nb.base_k);
+      const uint32_t a1 = Codes<T>::pair(y, nb.mask, nb.base_k), a3 = Codes<T>::pair(y >> 4, nb.mask, nb.base_k);
 #pragma unroll
       for (int t = 0; t < NT; ++t) mma<T>(acc[t], a0, a1, a2, a3, q.f[t][j * 4 + k][0], q.f[t][j * 4 + k][1]);
     }
@@ -394,11 +403,11 @@ AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int hea
   constexpr int H = NT * 8;
   for (int i = threadIdx.x; i < heads * (D / 4); i += kDecThreads) {
     const int h = i / (D / 4), d4 = i % (D / 4) * 4;
-    float m = -INFINITY, l = 0.f;
+    float m = kLowest, l = 0.f;
     for (int w = 0; w < nact; ++w) m = fmaxf(m, ml[w * H + h]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = 0; w < nact; ++w) {
-      const float f = m == -INFINITY ? 1.f : fast_exp2(ml[w * H + h] - m);
+      const float f = fast_exp2(ml[w * H + h] - m);
       l = fmaf(ml[(kWarps + w) * H + h], f, l);
       const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)w * H + h) * D + d4);
       o.x = fmaf(v.x, f, o.x);
@@ -437,7 +446,7 @@ struct Acc {
       for (int i = 0; i < G * 4; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < G; ++j) zo[t][j][0] = zo[t][j][1] = 0.f;
-      m[t][0] = m[t][1] = -INFINITY;
+      m[t][0] = m[t][1] = kLowest;
       l[t][0] = l[t][1] = 0.f;
     }
   }
@@ -447,14 +456,14 @@ struct Acc {
 // than 16): the others weigh nothing, whatever their bytes hold.
 template <typename T, int D, int NT, bool kTail>
 AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                          float scale_log2, int left, int lane) {
+                          float scale_log2, const Nibbles& nb, int left, int lane) {
   using R = Ring<D>;
   constexpr int G = D / kGroup;
   // bf16 results take p * step rounded to bf16; fp16 ones take a second,
   // low part as well, so that the output's own rounding stays the larger.
   constexpr int kParts = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
   float s[NT][4];
-  tile_logits<T, D, NT>(s, q, stage, at, scale_log2);
+  tile_logits<T, D, NT>(s, q, stage, at, scale_log2, nb);
   const int r0 = tile_row(lane >> 2);
   const bool in0 = !kTail || r0 < left, in1 = !kTail || r0 + 8 < left;
   bool grow = false;
@@ -474,7 +483,7 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         mx = fmaxf(mx, acc.m[t][e]);
-        const float f = mx == -INFINITY ? 1.f : fast_exp2(acc.m[t][e] - mx);
+        const float f = fast_exp2(acc.m[t][e] - mx);
         acc.m[t][e] = mx;
         acc.l[t][e] *= f;
 #pragma unroll
@@ -491,8 +500,7 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // a maximum of -inf is left only where every logit so far is -inf or NaN
-      s[t][i] = fast_exp2(s[t][i] - (acc.m[t][i & 1] == -INFINITY ? 0.f : acc.m[t][i & 1]));
+      s[t][i] = fast_exp2(s[t][i] - acc.m[t][i & 1]);
       acc.l[t][i & 1] += s[t][i];
     }
   }
@@ -526,8 +534,8 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
     const uint32_t x2 = __byte_perm(w2, w3, 0x5410), x3 = __byte_perm(w2, w3, 0x7632);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t a0 = Codes<__nv_bfloat16>::pair(x0 >> (4 * i)), a1 = Codes<__nv_bfloat16>::pair(x1 >> (4 * i));
-      const uint32_t a2 = Codes<__nv_bfloat16>::pair(x2 >> (4 * i)), a3 = Codes<__nv_bfloat16>::pair(x3 >> (4 * i));
+      const uint32_t a0 = Codes<__nv_bfloat16>::pair(x0 >> (4 * i), nb.mask, nb.base_v), a1 = Codes<__nv_bfloat16>::pair(x1 >> (4 * i), nb.mask, nb.base_v);
+      const uint32_t a2 = Codes<__nv_bfloat16>::pair(x2 >> (4 * i), nb.mask, nb.base_v), a3 = Codes<__nv_bfloat16>::pair(x3 >> (4 * i), nb.mask, nb.base_v);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -553,6 +561,7 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   const int g = lane >> 2, c = lane & 3;
   const int heads_v = p.kv_heads * p.chunks;
   const Places<D> place(lane);
+  const Nibbles nb{p.nibble_mask, p.base_k, p.base_v};
 
   int64_t at = 0, end = 1;  // direct: one (sequence, head chunk) per CTA
   if (!p.direct) {
@@ -615,9 +624,9 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
       copy_next(into);  // into the stage that the previous tile has left
       const int left = n - tile * kTile;
       if (left >= kTile)
-        take_tile<T, D, NT, false>(acc, q, st, place, p.scale_log2, left, lane);
+        take_tile<T, D, NT, false>(acc, q, st, place, p.scale_log2, nb, left, lane);
       else
-        take_tile<T, D, NT, true>(acc, q, st, place, p.scale_log2, left, lane);
+        take_tile<T, D, NT, true>(acc, q, st, place, p.scale_log2, nb, left, lane);
       into = st;
       st = st == base + kLast ? base : st + R::kStageBytes;
       __syncwarp();  // every lane is done with this stage before it is refilled
@@ -708,14 +717,14 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
   const int64_t c0 = start / share, c1 = (start + tiles - 1) / share;
   if (c0 == c1) return;  // one CTA had all of it and wrote the result
   auto slot = [&](int64_t c) { return (2 * c + (c == c0 ? 1 : 0)) * heads_chunk + h; };
-  float m = -INFINITY;
+  float m = kLowest;
   for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, p.part_ml[slot(c) * 2]);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
   const int d0 = threadIdx.x, d1 = threadIdx.x + 128;
 #pragma unroll 4
   for (int64_t c = c0; c <= c1; ++c) {
     const int64_t sl = slot(c);
-    const float f = m == -INFINITY ? 1.f : fast_exp2(p.part_ml[sl * 2] - m);
+    const float f = fast_exp2(p.part_ml[sl * 2] - m);
     l = fmaf(p.part_ml[sl * 2 + 1], f, l);
     if (d0 < dim) o0 = fmaf(p.part_o[sl * dim + d0], f, o0);
     if (d1 < dim) o1 = fmaf(p.part_o[sl * dim + d1], f, o1);
@@ -740,6 +749,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
   const int c = lane & 3, r0 = tile_row(lane >> 2);
   const int heads_v = p.kv_heads * p.chunks;
   const Places<D> place(lane);
+  const Nibbles nb{p.nibble_mask, p.base_k, p.base_v};
   cost_prefix(p, cum, s_warp);
   const int64_t total = (int64_t)cum[p.batch] * heads_v;
   const int64_t share = share_of(total, gridDim.x);
@@ -793,7 +803,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
       __syncwarp();
       copy_next(into);
       float s[NT][4];
-      tile_logits<T, D, NT>(s, q, st, place, p.scale_log2);
+      tile_logits<T, D, NT>(s, q, st, place, p.scale_log2, nb);
       into = st;
       st = st == base + kLast ? base : st + R::kHalf;
       float w0 = 0.f, w1 = 0.f;
@@ -863,7 +873,10 @@ cudaError_t run(const Kv4DecodeParams& p, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t dispatch(const Kv4DecodeParams& p, cudaStream_t s) {
+cudaError_t dispatch(Kv4DecodeParams p, cudaStream_t s) {
+  p.nibble_mask = 0x000F000Fu;
+  p.base_k = Codes<T>::kBase;
+  p.base_v = Codes<__nv_bfloat16>::kBase;
   const bool wide = p.head_tiles == 2;
   switch (p.dim) {
     case 64: return wide ? run<T, 64, 2>(p, s) : run<T, 64, 1>(p, s);

@@ -404,8 +404,10 @@ struct Kv4DecodeParams {
   int* status;                // or null
   int batch, heads, kv_heads, dim, block_size, num_blocks, max_blocks;
   int head_tiles, chunks, ctas, direct;  // from the plan
-  int ring_bytes;             // set by the launcher
   float scale_log2;
+  // set by the launcher
+  int ring_bytes;
+  uint32_t nibble_mask, base_k, base_v;
 };
 struct Kv4Plan {
   int head_tiles;  // 8 or 16 query heads of a KV head per pass
