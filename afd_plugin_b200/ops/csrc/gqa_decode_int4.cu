@@ -6,11 +6,10 @@
 // With codes shifted to c - 8 (and zero to zero + 8 step) the products split:
 //   q . k_t = sum_groups step_t,j * (q_j . c_t,j) + zero_t,j * sum(q_j)
 //   o       = sum_groups (p_t step_t,j) c_t,j + p_t zero_t,j
-// so the tensor cores multiply q (exact in its own type) and p * step with
-// small integers (exact in bf16 / fp16), and the scales stay outside in fp32.
-// p * step is rounded to bf16 for the second product (8 bits: fp16 would not
-// hold the range of the steps); everything else, the running maximum and sum
-// included, is fp32.
+// so the tensor cores multiply q (scaled by a power of two per head, exact in
+// fp16) and p * step (rounded to fp16's 11 bits, see take_tile) with small
+// integers, and the scales stay outside in fp32, as do the running maximum and
+// sum.
 //
 // What bounds it: the packed rows, 144 B per position and KV head at D = 128,
 // at the HBM rate.  A warp unpacks the codes it needs straight into MMA
@@ -47,6 +46,7 @@ constexpr int kStages = 4;
 constexpr int kDecThreads = kWarps * 32;
 constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
+constexpr float kStepTop = 512.f;    // scaled steps stay below this (times 2^kLazy: fp16 factors below 2^15)
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
 // What a piece costs beside its tiles (pipeline fill, query, merge), in tiles.
 constexpr int kPieceCost = 4;
@@ -73,45 +73,45 @@ AFD_DEVICE constexpr int swz(int row, int chunk) {
 }
 template <int D> constexpr int kRow4 = D == 256 ? 64 : (D == 128 ? 32 : 0);
 
-// Nibbles 0 and 4 of w as two values c - 8 of T.  OR-ing a code into the
-// mantissa of 128 (bf16) or 1024 (fp16) adds it; the subtraction is exact.
-// Mask and base come from the kernel's parameters: as literals they would cost
-// two logic operations instead of one (an instruction takes one literal).
-template <typename T> struct Codes;
-template <> struct Codes<__nv_bfloat16> {
-  static constexpr uint32_t kBase = 0x43004300u;
-  static AFD_DEVICE uint32_t pair(uint32_t w, uint32_t mask, uint32_t base) {
-    const uint32_t m = (w & mask) | base;
-    __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), __floats2bfloat162_rn(136.f, 136.f));
-    return *reinterpret_cast<uint32_t*>(&v);
+// The 8 codes of a word as fp16 pairs c - 8: v[i] = codes i and i + 4.  OR-ing
+// a code into the mantissa of 1024 adds it (or 16 times it, from the nibble
+// above); one multiply-add brings it down, exactly.  Masks and base come from
+// the kernel's parameters: as literals they would cost two logic operations
+// each instead of one (an instruction takes one literal).
+struct Unpack {
+  uint32_t lo, hi, base;
+  AFD_DEVICE void operator()(uint32_t (&v)[4], uint32_t w) const {
+    const uint32_t x = w >> 8;
+    v[0] = sub((w & lo) | base);
+    v[1] = down((w & hi) | base);
+    v[2] = sub((x & lo) | base);
+    v[3] = down((x & hi) | base);
   }
-};
-template <> struct Codes<__half> {
-  static constexpr uint32_t kBase = 0x64006400u;
-  static AFD_DEVICE uint32_t pair(uint32_t w, uint32_t mask, uint32_t base) {
-    const uint32_t m = (w & mask) | base;
-    __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1032.f, 1032.f));
-    return *reinterpret_cast<uint32_t*>(&v);
+  static AFD_DEVICE uint32_t sub(uint32_t m) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
-};
-struct Nibbles {
-  uint32_t mask, base_k, base_v;
+  static AFD_DEVICE uint32_t down(uint32_t m) {
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&m), __floats2half2_rn(0.0625f, 0.0625f),
+                              __floats2half2_rn(-72.f, -72.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 };
 
-template <typename T> AFD_DEVICE void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1);
-template <> AFD_DEVICE void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <> AFD_DEVICE void mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
+AFD_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+AFD_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// 2^e of x's binary exponent e + `by`, from the encoding; zero, subnormal and
+// infinite x count as the nearest exponent that keeps the result and its
+// inverse finite.
+AFD_DEVICE int exponent_of(float x) { return min(max((int)(__float_as_uint(x) >> 23) & 255, 40), 214) - 127; }
+AFD_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // 8x8 transpose of 16-bit values held one row pair per lane.
 AFD_DEVICE uint32_t transpose8(uint32_t v) {
@@ -192,7 +192,10 @@ AFD_DEVICE void cost_prefix(const Kv4DecodeParams& p, int* cum, int* warp_sums) 
   __syncthreads();
 }
 
-// The share of the batch's cost a CTA takes (the same expression wherever it is needed).
+// The share of the batch's cost a CTA takes (the same expression wherever it is
+// needed).  One wave of CTAs: two or four waves of shorter shares measured 2 and
+// 11% slower at 16 sequences of 50 - 131 K positions, each CTA's start costing
+// more than the evener finish gains.
 AFD_DEVICE int64_t share_of(int64_t total, int ctas) {
   const int64_t s = (total + ctas - 1) / ctas;
   return s < kMinShare + kPieceCost ? kMinShare + kPieceCost : s;
@@ -236,10 +239,9 @@ struct TileWalk {
   const int32_t* table;
   uint32_t block_codes, block_pairs;  // bytes of a block's codes and pairs
   int pg, in, per_block, step_pg, step_in, num_blocks, blk;
-  int* status;
 
   AFD_DEVICE TileWalk(const Kv4DecodeParams& p, int b, int kv_head, int first, int lane)
-      : table(p.block_table + (int64_t)b * p.table_stride), num_blocks(p.num_blocks), status(p.status) {
+      : table(p.block_table + (int64_t)b * p.table_stride), num_blocks(p.num_blocks) {
     const uint32_t rows = (uint32_t)kv_head * p.block_size;
     kc = p.k_codes + (size_t)rows * (D / 2) + lane * 16;
     vc = p.v_codes + (size_t)rows * (D / 2) + lane * 16;
@@ -254,15 +256,8 @@ struct TileWalk {
     step_pg = kWarps / per_block;
     step_in = kWarps - step_pg * per_block;
   }
-  // Reads the block id of the current tile.  One outside the pool is reported
-  // and replaced by the padding block.
-  AFD_DEVICE void fetch() {
-    blk = table[pg];
-    if ((unsigned)blk >= (unsigned)num_blocks) {
-      if (status != nullptr) atomicExch(status, kStatusBadIndex);
-      blk = 0;
-    }
-  }
+  // Reads the block id of the current tile (see check_blocks for bad ones).
+  AFD_DEVICE void fetch() { blk = (int)min((unsigned)table[pg], (unsigned)num_blocks - 1u); }
   AFD_DEVICE void advance() {
     pg += step_pg;
     in += step_in;
@@ -289,6 +284,15 @@ struct TileWalk {
   }
 };
 
+// Reports block ids of tiles [t0, t1) that lie outside the pool (the walk reads
+// the pool's last block in their place).
+AFD_DEVICE void check_blocks(const Kv4DecodeParams& p, int b, int t0, int t1) {
+  const int32_t* table = p.block_table + (int64_t)b * p.table_stride;
+  const int per_block = p.block_size / kTile;
+  for (int pg = t0 / per_block + (int)threadIdx.x; pg * per_block < t1; pg += kDecThreads)
+    if ((unsigned)table[pg] >= (unsigned)p.num_blocks && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
+}
+
 // Where this lane copies to and reads from inside a stage.
 template <int D>
 struct Places {
@@ -305,35 +309,51 @@ struct Places {
 
 // The query heads of one chunk as B operands, and their sums per dim group.
 // Column n of tile t is head t * 8 + n of the chunk (zero beyond `heads`).
+// Each head is scaled by a power of two, its largest value to [2^14, 2^15):
+// a bf16 value fits fp16 exactly then, down to 2^-31 of the head's largest
+// (an fp16 one down to 2^-28).
 template <typename T, int D, int NT>
 struct Query {
   static constexpr int G = D / kGroup;
   uint32_t f[NT][G * 4][2];
   float sum[NT][G][2];  // of heads 2c, 2c + 1, times scale * log2(e)
+  float unit[NT][2];    // what one unit of the scaled q . codes stands for, in the same
 
   AFD_DEVICE void load(const T* sq, float scale_log2, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const T* row = sq + (t * 8 + g) * D + c * 16;
+      float amax = 0.f;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
         float acc = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // word k / 2, half k % 2
-          const T* at = row + j * kGroup + (k >> 1) * 8 + (k & 1) * 2;
-          const T v[4] = {at[0], at[4], at[1], at[5]};
-          f[t][j * 4 + k][0] = reinterpret_cast<const uint16_t&>(v[0]) |
-                               (uint32_t) reinterpret_cast<const uint16_t&>(v[1]) << 16;
-          f[t][j * 4 + k][1] = reinterpret_cast<const uint16_t&>(v[2]) |
-                               (uint32_t) reinterpret_cast<const uint16_t&>(v[3]) << 16;
-          acc += (to_f32(v[0]) + to_f32(v[1])) + (to_f32(v[2]) + to_f32(v[3]));
+        for (int i = 0; i < 16; ++i) {
+          const float x = to_f32(row[j * kGroup + i]);
+          acc += x;
+          amax = fmaxf(amax, fabsf(x));
         }
         acc += __shfl_xor_sync(0xffffffffu, acc, 1);
         acc += __shfl_xor_sync(0xffffffffu, acc, 2);
         acc *= scale_log2;
         sum[t][j][0] = __shfl_sync(0xffffffffu, acc, c * 8);
         sum[t][j][1] = __shfl_sync(0xffffffffu, acc, c * 8 + 4);
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int e = 14 - exponent_of(amax);
+      const float up = pow2(e), down = pow2(-e) * scale_log2;
+      unit[t][0] = __shfl_sync(0xffffffffu, down, c * 8);
+      unit[t][1] = __shfl_sync(0xffffffffu, down, c * 8 + 4);
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // word k / 2, code pairs 2 (k % 2) and 2 (k % 2) + 1
+          const T* at = row + j * kGroup + (k >> 1) * 8 + (k & 1) * 2;
+          f[t][j * 4 + k][0] = pack_f16(to_f32(at[0]) * up, to_f32(at[4]) * up);
+          f[t][j * 4 + k][1] = pack_f16(to_f32(at[1]) * up, to_f32(at[5]) * up);
+        }
       }
     }
   }
@@ -343,11 +363,12 @@ struct Query {
 // (i = 2, 3), heads t * 8 + 2c + (i & 1); in the log2 domain.
 template <typename T, int D, int NT>
 AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                            float scale_log2, const Nibbles& nb) {
+                            const Unpack& codes, uint32_t shl16) {
   constexpr int G = D / kGroup;
   uint32_t p0[G], p1[G];
   lds_pairs<G>(p0, stage + at.pair);
   lds_pairs<G>(p1, stage + at.pair + 8 * G * 4);
+  float z[NT][4];
 #pragma unroll
   for (int j = 0; j < G; ++j) {
     uint32_t w0[2], w1[2];
@@ -358,31 +379,32 @@ AFD_DEVICE void tile_logits(float (&s)[NT][4], const Query<T, D, NT>& q, uint32_
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t x = w0[k >> 1] >> ((k & 1) * 8), y = w1[k >> 1] >> ((k & 1) * 8);
-      const uint32_t a0 = Codes<T>::pair(x, nb.mask, nb.base_k), a2 = Codes<T>::pair(x >> 4, nb.mask, nb.base_k);
-      const uint32_t a1 = Codes<T>::pair(y, nb.mask, nb.base_k), a3 = Codes<T>::pair(y >> 4, nb.mask, nb.base_k);
+    for (int k = 0; k < 2; ++k) {
+      uint32_t x[4], y[4];
+      codes(x, w0[k]);
+      codes(y, w1[k]);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) mma<T>(acc[t], a0, a1, a2, a3, q.f[t][j * 4 + k][0], q.f[t][j * 4 + k][1]);
+      for (int t = 0; t < NT; ++t) {
+        mma_f16(acc[t], x[0], y[0], x[1], y[1], q.f[t][j * 4 + 2 * k][0], q.f[t][j * 4 + 2 * k][1]);
+        mma_f16(acc[t], x[2], y[2], x[3], y[3], q.f[t][j * 4 + 2 * k + 1][0], q.f[t][j * 4 + 2 * k + 1][1]);
+      }
     }
-    const float st0 = pair_step(p0[j]), st1 = pair_step(p1[j]);
+    const float st0 = pair_step(p0[j], shl16), st1 = pair_step(p1[j], shl16);
     const float z0 = fmaf(8.f, st0, pair_zero(p0[j])), z1 = fmaf(8.f, st1, pair_zero(p1[j]));
-    const float m0 = st0 * scale_log2, m1 = st1 * scale_log2;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if (j == 0) {
-        s[t][0] = fmaf(m0, acc[t][0], z0 * q.sum[t][j][0]);
-        s[t][1] = fmaf(m0, acc[t][1], z0 * q.sum[t][j][1]);
-        s[t][2] = fmaf(m1, acc[t][2], z1 * q.sum[t][j][0]);
-        s[t][3] = fmaf(m1, acc[t][3], z1 * q.sum[t][j][1]);
-      } else {
-        s[t][0] = fmaf(m0, acc[t][0], fmaf(z0, q.sum[t][j][0], s[t][0]));
-        s[t][1] = fmaf(m0, acc[t][1], fmaf(z0, q.sum[t][j][1], s[t][1]));
-        s[t][2] = fmaf(m1, acc[t][2], fmaf(z1, q.sum[t][j][0], s[t][2]));
-        s[t][3] = fmaf(m1, acc[t][3], fmaf(z1, q.sum[t][j][1], s[t][3]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float st = i < 2 ? st0 : st1, zz = i < 2 ? z0 : z1;
+        s[t][i] = j == 0 ? st * acc[t][i] : fmaf(st, acc[t][i], s[t][i]);
+        z[t][i] = j == 0 ? zz * q.sum[t][j][i & 1] : fmaf(zz, q.sum[t][j][i & 1], z[t][i]);
       }
     }
   }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = fmaf(s[t][i], q.unit[t][i & 1], z[t][i]);
 }
 
 // Stage the chunk's query heads in shared memory (rows beyond them zero).
@@ -439,6 +461,7 @@ template <int D, int NT>
 struct Acc {
   static constexpr int G = D / kGroup;
   float o[NT][G * 4][4], zo[NT][G][2], m[NT][2], l[NT][2];
+  float scale[G];  // power of two that o's group j is multiplied by
   AFD_DEVICE void clear() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -449,24 +472,42 @@ struct Acc {
       m[t][0] = m[t][1] = kLowest;
       l[t][0] = l[t][1] = 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < G; ++j) scale[j] = pow2(87);
   }
 };
 
 // One tile in a stage of the ring.  `left` positions of it exist (kTail: fewer
 // than 16): the others weigh nothing, whatever their bytes hold.
+//
+// The second product takes p * step in fp16, 11 bits.  p is at most 2^kLazy,
+// and a power of two per dim group (kept per warp, lowered when a larger step
+// comes) holds the steps below 2^9, so the factors stay below 2^15.  A step
+// that set the scale gets 2^5 at least: factors keep full precision down to
+// 2^-19 of it, and below that are off by at most 2^-30 of it.
 template <typename T, int D, int NT, bool kTail>
 AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                          float scale_log2, const Nibbles& nb, int left, int lane) {
+                          const Unpack& codes, uint32_t shl16, int left, int lane) {
   using R = Ring<D>;
   constexpr int G = D / kGroup;
-  // bf16 results take p * step rounded to bf16; fp16 ones take a second,
-  // low part as well, so that the output's own rounding stays the larger.
-  constexpr int kParts = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
   float s[NT][4];
-  tile_logits<T, D, NT>(s, q, stage, at, scale_log2, nb);
+  tile_logits<T, D, NT>(s, q, stage, at, codes, shl16);
   const int r0 = tile_row(lane >> 2);
   const bool in0 = !kTail || r0 < left, in1 = !kTail || r0 + 8 < left;
+  uint32_t p0[G], p1[G];
+  lds_pairs<G>(p0, stage + R::kHalf + at.pair);
+  lds_pairs<G>(p1, stage + R::kHalf + at.pair + 8 * G * 4);
+  // positions past the end hold anything: their factors are zero, not 0 * that
+  float st0[G], st1[G], k0[G], k1[G];
   bool grow = false;
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    st0[j] = in0 ? pair_step(p0[j], shl16) : 0.f;
+    st1[j] = in1 ? pair_step(p1[j], shl16) : 0.f;
+    k0[j] = st0[j] * acc.scale[j];
+    k1[j] = st1[j] * acc.scale[j];
+    grow |= fmaxf(k0[j], k1[j]) >= kStepTop;
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (!in0) s[t][0] = s[t][1] = -INFINITY;
@@ -474,24 +515,40 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
     grow |= fmaxf(s[t][0], s[t][2]) > acc.m[t][0] + kLazy || fmaxf(s[t][1], s[t][3]) > acc.m[t][1] + kLazy;
   }
   if (__any_sync(0xffffffffu, grow)) {
+    float by[G];  // what o's scale changes by
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      float mx = fmaxf(st0[j], st1[j]);
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      by[j] = 1.f;
+      if (mx * acc.scale[j] >= kStepTop) {  // the largest step to [2^5, 2^6): three binades of room
+        const int e = 5 - exponent_of(mx);
+        by[j] = pow2(e) / acc.scale[j];
+        acc.scale[j] = pow2(e);
+        k0[j] = st0[j] * acc.scale[j];
+        k1[j] = st1[j] * acc.scale[j];
+      }
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float mx = fmaxf(s[t][e], s[t][2 + e]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
         mx = fmaxf(mx, acc.m[t][e]);
         const float f = fast_exp2(acc.m[t][e] - mx);
         acc.m[t][e] = mx;
         acc.l[t][e] *= f;
 #pragma unroll
-        for (int j = 0; j < G; ++j) acc.zo[t][j][e] *= f;
+        for (int j = 0; j < G; ++j) {
+          acc.zo[t][j][e] *= f;
 #pragma unroll
-        for (int i = 0; i < G * 4; ++i) {
-          acc.o[t][i][e] *= f;
-          acc.o[t][i][2 + e] *= f;
+          for (int i = 0; i < 4; ++i) {
+            acc.o[t][j * 4 + i][e] *= f * by[j];
+            acc.o[t][j * 4 + i][2 + e] *= f * by[j];
+          }
         }
       }
     }
@@ -505,48 +562,39 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
     }
   }
   // P V: the probabilities, scaled per dim group, are the B operand.
-  uint32_t p0[G], p1[G];
-  lds_pairs<G>(p0, stage + R::kHalf + at.pair);
-  lds_pairs<G>(p1, stage + R::kHalf + at.pair + 8 * G * 4);
 #pragma unroll
   for (int j = 0; j < G; ++j) {
-    // positions past the end hold anything: their factors are zero, not 0 * that
-    const float st0 = in0 ? pair_step(p0[j]) : 0.f, st1 = in1 ? pair_step(p1[j]) : 0.f;
-    const float z0 = in0 ? fmaf(8.f, st0, pair_zero(p0[j])) : 0.f, z1 = in1 ? fmaf(8.f, st1, pair_zero(p1[j])) : 0.f;
-    uint32_t b[NT][kParts][2];
+    const float z0 = in0 ? fmaf(8.f, st0[j], pair_zero(p0[j])) : 0.f;
+    const float z1 = in1 ? fmaf(8.f, st1[j], pair_zero(p1[j])) : 0.f;
+    uint32_t b[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       acc.zo[t][j][0] = fmaf(s[t][0], z0, fmaf(s[t][2], z1, acc.zo[t][j][0]));
       acc.zo[t][j][1] = fmaf(s[t][1], z0, fmaf(s[t][3], z1, acc.zo[t][j][1]));
-      const float x[4] = {s[t][0] * st0, s[t][1] * st0, s[t][2] * st1, s[t][3] * st1};
-      const uint32_t h0 = pack_bf16(x[0], x[1]), h1 = pack_bf16(x[2], x[3]);
-      b[t][0][0] = transpose8(h0);
-      b[t][0][1] = transpose8(h1);
-      if constexpr (kParts == 2) {
-        b[t][1][0] = transpose8(pack_bf16(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xFFFF0000u)));
-        b[t][1][1] = transpose8(pack_bf16(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xFFFF0000u)));
-      }
+      b[t][0] = transpose8(pack_f16(s[t][0] * k0[j], s[t][1] * k0[j]));
+      b[t][1] = transpose8(pack_f16(s[t][2] * k1[j], s[t][3] * k1[j]));
     }
     // k indices 2c, 2c + 1, 2c + 8, 2c + 9 are rows c, c + 4, c + 8, c + 12
     const uint32_t even = (stage + at.v) ^ (j * 32), odd = (even ^ kRow4<D>) + 4 * (D / 2);
     const uint32_t w0 = lds32(even), w1 = lds32(odd), w2 = lds32(even + 8 * (D / 2)), w3 = lds32(odd + 8 * (D / 2));
-    const uint32_t x0 = __byte_perm(w0, w1, 0x5410), x1 = __byte_perm(w0, w1, 0x7632);
-    const uint32_t x2 = __byte_perm(w2, w3, 0x5410), x3 = __byte_perm(w2, w3, 0x7632);
+    // codes 0 .. 3 (dims) of two positions, then codes 4 .. 7
+    uint32_t x0[4], x1[4], x2[4], x3[4];
+    codes(x0, __byte_perm(w0, w1, 0x5410));
+    codes(x1, __byte_perm(w0, w1, 0x7632));
+    codes(x2, __byte_perm(w2, w3, 0x5410));
+    codes(x3, __byte_perm(w2, w3, 0x7632));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a0 = Codes<__nv_bfloat16>::pair(x0 >> (4 * i), nb.mask, nb.base_v), a1 = Codes<__nv_bfloat16>::pair(x1 >> (4 * i), nb.mask, nb.base_v);
-      const uint32_t a2 = Codes<__nv_bfloat16>::pair(x2 >> (4 * i), nb.mask, nb.base_v), a3 = Codes<__nv_bfloat16>::pair(x3 >> (4 * i), nb.mask, nb.base_v);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int u = 0; u < kParts; ++u)
-          mma<__nv_bfloat16>(acc.o[t][j * 4 + i], a0, a1, a2, a3, b[t][u][0], b[t][u][1]);
-    }
+      for (int t = 0; t < NT; ++t) mma_f16(acc.o[t][j * 4 + i], x0[i], x1[i], x2[i], x3[i], b[t][0], b[t][1]);
   }
 }
 
 // CTAs of kWarps warps that one SM holds (registers bound it).
-template <int D, int NT> constexpr int kResident = D * NT <= 128 ? 4 : 2;
+#ifndef RES
+#define RES 4
+#endif
+template <int D, int NT> constexpr int kResident = D * NT <= 128 ? RES : 2;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel(Kv4DecodeParams p) {
@@ -561,7 +609,7 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   const int g = lane >> 2, c = lane & 3;
   const int heads_v = p.kv_heads * p.chunks;
   const Places<D> place(lane);
-  const Nibbles nb{p.nibble_mask, p.base_k, p.base_v};
+  const Unpack codes{p.mask_lo, p.mask_hi, p.base_f16};
 
   int64_t at = 0, end = 1;  // direct: one (sequence, head chunk) per CTA
   if (!p.direct) {
@@ -610,6 +658,7 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * R::kStageBytes);
     stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
+    check_blocks(p, pc.b, pc.t0, pc.t1);
     __syncthreads();
     Query<T, D, NT> q;
     q.load(sq, p.scale_log2, lane);
@@ -624,9 +673,9 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
       copy_next(into);  // into the stage that the previous tile has left
       const int left = n - tile * kTile;
       if (left >= kTile)
-        take_tile<T, D, NT, false>(acc, q, st, place, p.scale_log2, nb, left, lane);
+        take_tile<T, D, NT, false>(acc, q, st, place, codes, p.shl16, left, lane);
       else
-        take_tile<T, D, NT, true>(acc, q, st, place, p.scale_log2, nb, left, lane);
+        take_tile<T, D, NT, true>(acc, q, st, place, codes, p.shl16, left, lane);
       into = st;
       st = st == base + kLast ? base : st + R::kStageBytes;
       __syncwarp();  // every lane is done with this stage before it is refilled
@@ -659,11 +708,13 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
 #pragma unroll
           for (int j = 0; j < G; ++j) {
             const auto& o = acc.o[t];
-            *reinterpret_cast<float4*>(to + j * kGroup) = make_float4(
-                o[j * 4][e] + z[j], o[j * 4 + 1][e] + z[j], o[j * 4 + 2][e] + z[j], o[j * 4 + 3][e] + z[j]);
+            const float u = 1.f / acc.scale[j];
+            *reinterpret_cast<float4*>(to + j * kGroup) =
+                make_float4(fmaf(o[j * 4][e], u, z[j]), fmaf(o[j * 4 + 1][e], u, z[j]), fmaf(o[j * 4 + 2][e], u, z[j]),
+                            fmaf(o[j * 4 + 3][e], u, z[j]));
             *reinterpret_cast<float4*>(to + j * kGroup + 4) =
-                make_float4(o[j * 4][2 + e] + z[j], o[j * 4 + 1][2 + e] + z[j], o[j * 4 + 2][2 + e] + z[j],
-                            o[j * 4 + 3][2 + e] + z[j]);
+                make_float4(fmaf(o[j * 4][2 + e], u, z[j]), fmaf(o[j * 4 + 1][2 + e], u, z[j]),
+                            fmaf(o[j * 4 + 2][2 + e], u, z[j]), fmaf(o[j * 4 + 3][2 + e], u, z[j]));
           }
         }
       }
@@ -749,7 +800,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
   const int c = lane & 3, r0 = tile_row(lane >> 2);
   const int heads_v = p.kv_heads * p.chunks;
   const Places<D> place(lane);
-  const Nibbles nb{p.nibble_mask, p.base_k, p.base_v};
+  const Unpack codes{p.mask_lo, p.mask_hi, p.base_f16};
   cost_prefix(p, cum, s_warp);
   const int64_t total = (int64_t)cum[p.batch] * heads_v;
   const int64_t share = share_of(total, gridDim.x);
@@ -803,7 +854,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
       __syncwarp();
       copy_next(into);
       float s[NT][4];
-      tile_logits<T, D, NT>(s, q, st, place, p.scale_log2, nb);
+      tile_logits<T, D, NT>(s, q, st, place, codes, p.shl16);
       into = st;
       st = st == base + kLast ? base : st + R::kHalf;
       float w0 = 0.f, w1 = 0.f;
@@ -874,9 +925,10 @@ cudaError_t run(const Kv4DecodeParams& p, cudaStream_t s) {
 
 template <typename T>
 cudaError_t dispatch(Kv4DecodeParams p, cudaStream_t s) {
-  p.nibble_mask = 0x000F000Fu;
-  p.base_k = Codes<T>::kBase;
-  p.base_v = Codes<__nv_bfloat16>::kBase;
+  p.mask_lo = 0x000F000Fu;
+  p.mask_hi = 0x00F000F0u;
+  p.base_f16 = 0x64006400u;
+  p.shl16 = 65536u;
   const bool wide = p.head_tiles == 2;
   switch (p.dim) {
     case 64: return wide ? run<T, 64, 2>(p, s) : run<T, 64, 1>(p, s);
@@ -901,7 +953,7 @@ Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len
   const int64_t items = (int64_t)batch * kv_heads * plan.chunks;
   constexpr int kDirectTiles = 32;
   plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
-  const int resident = dim * plan.head_tiles <= 128 ? 4 : 2;  // kResident
+  const int resident = dim * plan.head_tiles <= 128 ? RES : 2;  // kResident
   plan.ctas = plan.direct ? (int)items : resident * device_sm_count();
   plan.max_batch = kv4::kMaxBatch;
   return plan;

@@ -27,6 +27,8 @@ AFD_DEVICE float bf16_down(float x) {
 
 // The low / high half of a (step, zero) pair as fp32.
 AFD_DEVICE float pair_step(uint32_t p) { return __uint_as_float(p << 16); }
+// The same by a product with 65536, for kernels whose logic pipe is the busy one.
+AFD_DEVICE float pair_step(uint32_t p, uint32_t shl16) { return __uint_as_float(p * shl16); }
 AFD_DEVICE float pair_zero(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
 }  // namespace kv4

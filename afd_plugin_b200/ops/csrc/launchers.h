@@ -407,7 +407,7 @@ struct Kv4DecodeParams {
   float scale_log2;
   // set by the launcher
   int ring_bytes;
-  uint32_t nibble_mask, base_k, base_v;
+  uint32_t mask_lo, mask_hi, base_f16, shl16;
 };
 struct Kv4Plan {
   int head_tiles;  // 8 or 16 query heads of a KV head per pass
