@@ -42,7 +42,8 @@ namespace kv4 {
 
 constexpr int kTile = 16;
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 3;       // of kTiles tiles each
+constexpr int kScoreStages = 4;  // of one tile's K
 constexpr int kDecThreads = kWarps * 32;
 constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
@@ -71,6 +72,12 @@ AFD_DEVICE constexpr int swz(int row, int chunk) {
   if (D == 128) return chunk ^ ((((row >> 1) ^ (row >> 2)) & 1) << 1);
   return chunk;
 }
+// Tiles a warp takes at once: two where the registers allow it, so that their
+// chains of dependent operations interleave.
+template <int D, int NT> constexpr int kTiles = D * NT <= 128 ? 2 : 1;
+// CTAs one SM holds (their registers bound it).  Measured at 16 sequences of
+// 50 - 131 K positions, D = 128: see the launcher.
+template <int D, int NT> constexpr int kResident = D * NT <= 128 ? 3 : 2;
 template <int D> constexpr int kRow4 = D == 256 ? 64 : (D == 128 ? 32 : 0);
 
 // The 8 codes of a word as fp16 pairs c - 8: v[i] = codes i and i + 4.  OR-ing
@@ -231,17 +238,18 @@ AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, in
   return pc;
 }
 
-// A warp's walk over the tiles of one (sequence, KV head) in the cache, every
-// kWarps-th tile from `first` on.  Block ids are fetched one tile ahead.
-template <int D>
+// A warp's walk over the tiles of one (sequence, KV head) in the cache: U
+// neighbouring tiles from `first` on, then those U * kWarps further, and so on.
+// Block ids are fetched one step ahead.
+template <int D, int U>
 struct TileWalk {
   const uint8_t *kc, *vc, *sc;  // this lane's bytes of the head's first row: K codes, V codes, pairs
   const int32_t* table;
   uint32_t block_codes, block_pairs;  // bytes of a block's codes and pairs
-  int pg, in, per_block, step_pg, step_in, num_blocks, blk;
+  int pg, in, per_block, last_block, blk[U];
 
   AFD_DEVICE TileWalk(const Kv4DecodeParams& p, int b, int kv_head, int first, int lane)
-      : table(p.block_table + (int64_t)b * p.table_stride), num_blocks(p.num_blocks) {
+      : table(p.block_table + (int64_t)b * p.table_stride), last_block(p.num_blocks - 1) {
     const uint32_t rows = (uint32_t)kv_head * p.block_size;
     kc = p.k_codes + (size_t)rows * (D / 2) + lane * 16;
     vc = p.v_codes + (size_t)rows * (D / 2) + lane * 16;
@@ -253,34 +261,46 @@ struct TileWalk {
     per_block = p.block_size / kTile;
     pg = first / per_block;
     in = first - pg * per_block;
-    step_pg = kWarps / per_block;
-    step_in = kWarps - step_pg * per_block;
   }
-  // Reads the block id of the current tile (see check_blocks for bad ones).
-  AFD_DEVICE void fetch() { blk = (int)min((unsigned)table[pg], (unsigned)num_blocks - 1u); }
+  // Page and place in it of the step's u-th tile.
+  AFD_DEVICE void at(int u, int& page, int& place) const {
+    const bool over = in + u >= per_block;  // u <= 1
+    page = pg + over;
+    place = over ? in + u - per_block : in + u;
+  }
+  // Reads the block ids of the step's first `n` tiles (see check_blocks for bad ones).
+  AFD_DEVICE void fetch(int n) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int page, place;
+      at(u, page, place);
+      if (u < n) blk[u] = (int)min((unsigned)table[page], (unsigned)last_block);
+    }
+  }
   AFD_DEVICE void advance() {
-    pg += step_pg;
-    in += step_in;
-    if (in >= per_block) {
+    in += U * kWarps;
+    while (in >= per_block) {
       in -= per_block;
       ++pg;
     }
   }
-  // `dst` / `dst_odd`: this lane's swizzled place in the stage (see lane_places).
+  // `dst`: this lane's swizzled place in a stage.
   template <bool kWithV>
-  AFD_DEVICE void load(uint32_t stage, uint32_t dst, int lane) const {
+  AFD_DEVICE void load(int u, uint32_t stage, uint32_t dst, int lane) const {
     using R = Ring<D>;
-    const size_t off = (size_t)blk * block_codes + (uint32_t)(in * R::kCodes);
+    int page, place;
+    at(u, page, place);
+    const size_t off = (size_t)blk[u] * block_codes + (uint32_t)(place * R::kCodes);
 #pragma unroll
-    for (int u = 0; u < R::kCodes / 512; ++u) {
+    for (int i = 0; i < R::kCodes / 512; ++i) {
       // 32 chunks on: the row grows by 8 (D = 128) or 4 (D = 256)
-      const uint32_t to = stage + ((D == 256 && (u & 1)) ? dst ^ 64u : dst) + u * 512;
-      cp16(to, kc + off + u * 512);
-      if (kWithV) cp16(to + R::kHalf, vc + off + u * 512);
+      const uint32_t to = stage + ((D == 256 && (i & 1)) ? dst ^ 64u : dst) + i * 512;
+      cp16(to, kc + off + i * 512);
+      if (kWithV) cp16(to + R::kHalf, vc + off + i * 512);
     }
     if ((lane & 15) < R::kPairs / 16 && (kWithV || lane < 16))
       cp16(stage + R::kCodes + (lane < 16 ? 0 : R::kHalf) + (lane & 15) * 16,
-           sc + (size_t)blk * block_pairs + (uint32_t)(in * R::kPairs));
+           sc + (size_t)blk[u] * block_pairs + (uint32_t)(place * R::kPairs));
   }
 };
 
@@ -477,8 +497,9 @@ struct Acc {
   }
 };
 
-// One tile in a stage of the ring.  `left` positions of it exist (kTail: fewer
-// than 16): the others weigh nothing, whatever their bytes hold.
+// The tiles of one step, in a stage of the ring.  `left` positions from the
+// first tile on exist (kTail: fewer than the step's): the others weigh nothing,
+// whatever their bytes hold.
 //
 // The second product takes p * step in fp16, 11 bits.  p is at most 2^kLazy,
 // and a power of two per dim group (kept per warp, lowered when a larger step
@@ -486,39 +507,60 @@ struct Acc {
 // that set the scale gets 2^5 at least: factors keep full precision down to
 // 2^-19 of it, and below that are off by at most 2^-30 of it.
 template <typename T, int D, int NT, bool kTail>
-AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                          const Unpack& codes, uint32_t shl16, int left, int lane) {
+AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
+                           const Unpack& codes, uint32_t shl16, int left, int lane) {
   using R = Ring<D>;
-  constexpr int G = D / kGroup;
-  float s[NT][4];
-  tile_logits<T, D, NT>(s, q, stage, at, codes, shl16);
+  constexpr int G = D / kGroup, U = kTiles<D, NT>;
+  float s[U][NT][4];
+#pragma unroll
+  for (int u = 0; u < U; ++u) tile_logits<T, D, NT>(s[u], q, stage + u * R::kStageBytes, at, codes, shl16);
   const int r0 = tile_row(lane >> 2);
-  const bool in0 = !kTail || r0 < left, in1 = !kTail || r0 + 8 < left;
-  uint32_t p0[G], p1[G];
-  lds_pairs<G>(p0, stage + R::kHalf + at.pair);
-  lds_pairs<G>(p1, stage + R::kHalf + at.pair + 8 * G * 4);
-  // positions past the end hold anything: their factors are zero, not 0 * that
-  float st0[G], st1[G], k0[G], k1[G];
+  uint32_t pr[U][2][G];          // (step, zero) of rows r0 and r0 + 8
+  float st[U][2][G], k[U][2][G]; // their steps, and scaled
   bool grow = false;
 #pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      lds_pairs<G>(pr[u][r], stage + u * R::kStageBytes + R::kHalf + at.pair + r * 8 * G * 4);
+      const bool in = !kTail || u * kTile + r0 + r * 8 < left;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        // positions past the end hold anything: their factors are zero, not 0 * that
+        if (kTail && !in) pr[u][r][j] = 0;
+        st[u][r][j] = pair_step(pr[u][r][j], shl16);
+        k[u][r][j] = st[u][r][j] * acc.scale[j];
+      }
+      if (kTail && !in) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[u][t][2 * r] = s[u][t][2 * r + 1] = -INFINITY;
+      }
+    }
+  }
+#pragma unroll
   for (int j = 0; j < G; ++j) {
-    st0[j] = in0 ? pair_step(p0[j], shl16) : 0.f;
-    st1[j] = in1 ? pair_step(p1[j], shl16) : 0.f;
-    k0[j] = st0[j] * acc.scale[j];
-    k1[j] = st1[j] * acc.scale[j];
-    grow |= fmaxf(k0[j], k1[j]) >= kStepTop;
+    float mx = fmaxf(k[0][0][j], k[0][1][j]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, fmaxf(k[u][0][j], k[u][1][j]));
+    grow |= mx >= kStepTop;
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    if (!in0) s[t][0] = s[t][1] = -INFINITY;
-    if (!in1) s[t][2] = s[t][3] = -INFINITY;
-    grow |= fmaxf(s[t][0], s[t][2]) > acc.m[t][0] + kLazy || fmaxf(s[t][1], s[t][3]) > acc.m[t][1] + kLazy;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mx = fmaxf(s[0][t][e], s[0][t][2 + e]);
+#pragma unroll
+      for (int u = 1; u < U; ++u) mx = fmaxf(mx, fmaxf(s[u][t][e], s[u][t][2 + e]));
+      grow |= mx > acc.m[t][e] + kLazy;
+    }
   }
   if (__any_sync(0xffffffffu, grow)) {
     float by[G];  // what o's scale changes by
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-      float mx = fmaxf(st0[j], st1[j]);
+      float mx = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(st[u][0][j], st[u][1][j]));
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       by[j] = 1.f;
@@ -526,18 +568,21 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
         const int e = 5 - exponent_of(mx);
         by[j] = pow2(e) / acc.scale[j];
         acc.scale[j] = pow2(e);
-        k0[j] = st0[j] * acc.scale[j];
-        k1[j] = st1[j] * acc.scale[j];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) k[u][r][j] = st[u][r][j] * acc.scale[j];
       }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(s[t][e], s[t][2 + e]);
+        float mx = acc.m[t][e];
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(s[u][t][e], s[u][t][2 + e]));
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        mx = fmaxf(mx, acc.m[t][e]);
         const float f = fast_exp2(acc.m[t][e] - mx);
         acc.m[t][e] = mx;
         acc.l[t][e] *= f;
@@ -554,52 +599,51 @@ AFD_DEVICE void take_tile(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t st
     }
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[t][i] = fast_exp2(s[t][i] - acc.m[t][i & 1]);
-      acc.l[t][i & 1] += s[t][i];
-    }
-  }
-  // P V: the probabilities, scaled per dim group, are the B operand.
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    const float z0 = in0 ? fmaf(8.f, st0[j], pair_zero(p0[j])) : 0.f;
-    const float z1 = in1 ? fmaf(8.f, st1[j], pair_zero(p1[j])) : 0.f;
-    uint32_t b[NT][2];
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      acc.zo[t][j][0] = fmaf(s[t][0], z0, fmaf(s[t][2], z1, acc.zo[t][j][0]));
-      acc.zo[t][j][1] = fmaf(s[t][1], z0, fmaf(s[t][3], z1, acc.zo[t][j][1]));
-      b[t][0] = transpose8(pack_f16(s[t][0] * k0[j], s[t][1] * k0[j]));
-      b[t][1] = transpose8(pack_f16(s[t][2] * k1[j], s[t][3] * k1[j]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[u][t][i] = fast_exp2(s[u][t][i] - acc.m[t][i & 1]);
+        acc.l[t][i & 1] += s[u][t][i];
+      }
     }
-    // k indices 2c, 2c + 1, 2c + 8, 2c + 9 are rows c, c + 4, c + 8, c + 12
-    const uint32_t even = (stage + at.v) ^ (j * 32), odd = (even ^ kRow4<D>) + 4 * (D / 2);
-    const uint32_t w0 = lds32(even), w1 = lds32(odd), w2 = lds32(even + 8 * (D / 2)), w3 = lds32(odd + 8 * (D / 2));
-    // codes 0 .. 3 (dims) of two positions, then codes 4 .. 7
-    uint32_t x0[4], x1[4], x2[4], x3[4];
-    codes(x0, __byte_perm(w0, w1, 0x5410));
-    codes(x1, __byte_perm(w0, w1, 0x7632));
-    codes(x2, __byte_perm(w2, w3, 0x5410));
-    codes(x3, __byte_perm(w2, w3, 0x7632));
+    // P V: the probabilities, scaled per dim group, are the B operand.
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < G; ++j) {
+      const float z0 = fmaf(8.f, st[u][0][j], pair_zero(pr[u][0][j]));
+      const float z1 = fmaf(8.f, st[u][1][j], pair_zero(pr[u][1][j]));
+      uint32_t b[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) mma_f16(acc.o[t][j * 4 + i], x0[i], x1[i], x2[i], x3[i], b[t][0], b[t][1]);
+      for (int t = 0; t < NT; ++t) {
+        const float* p = s[u][t];
+        acc.zo[t][j][0] = fmaf(p[0], z0, fmaf(p[2], z1, acc.zo[t][j][0]));
+        acc.zo[t][j][1] = fmaf(p[1], z0, fmaf(p[3], z1, acc.zo[t][j][1]));
+        b[t][0] = transpose8(pack_f16(p[0] * k[u][0][j], p[1] * k[u][0][j]));
+        b[t][1] = transpose8(pack_f16(p[2] * k[u][1][j], p[3] * k[u][1][j]));
+      }
+      // k indices 2c, 2c + 1, 2c + 8, 2c + 9 are rows c, c + 4, c + 8, c + 12
+      const uint32_t even = ((stage + at.v) ^ (j * 32)) + u * R::kStageBytes;
+      const uint32_t odd = ((stage + at.v) ^ (j * 32) ^ kRow4<D>) + 4 * (D / 2) + u * R::kStageBytes;
+      const uint32_t w0 = lds32(even), w1 = lds32(odd), w2 = lds32(even + 8 * (D / 2)), w3 = lds32(odd + 8 * (D / 2));
+      // codes 0 .. 3 (dims) of two positions, then codes 4 .. 7
+      uint32_t x0[4], x1[4], x2[4], x3[4];
+      codes(x0, __byte_perm(w0, w1, 0x5410));
+      codes(x1, __byte_perm(w0, w1, 0x7632));
+      codes(x2, __byte_perm(w2, w3, 0x5410));
+      codes(x3, __byte_perm(w2, w3, 0x7632));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_f16(acc.o[t][j * 4 + i], x0[i], x1[i], x2[i], x3[i], b[t][0], b[t][1]);
+    }
   }
 }
-
-// CTAs of kWarps warps that one SM holds (registers bound it).
-#ifndef RES
-#define RES 4
-#endif
-template <int D, int NT> constexpr int kResident = D * NT <= 128 ? RES : 2;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel(Kv4DecodeParams p) {
   using R = Ring<D>;
-  constexpr int G = D / kGroup, H = NT * 8;
+  constexpr int G = D / kGroup, H = NT * 8, U = kTiles<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_warp[kWarps];
   __shared__ float s_ml[2 * kWarps * H];
@@ -640,23 +684,26 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
     const int h_in = pc.hv % p.chunks * H;
     const int heads = min(H, group - h_in);
     const int head0 = kv_head * group + h_in;
-    const uint32_t base = smem_u32(smem) + warp * kStages * R::kStageBytes;
+    constexpr uint32_t kStep = U * R::kStageBytes;
+    const uint32_t base = smem_u32(smem) + warp * kStages * kStep;
 
-    // Fill the ring.  Tiles of a piece are dealt to the warps in turn.
-    int issue = pc.t0 + warp;
-    TileWalk<D> walk(p, pc.b, kv_head, issue, lane);
-    if (issue < pc.t1) walk.fetch();
+    // Fill the ring.  Steps of U tiles of a piece are dealt to the warps in turn.
+    int issue = pc.t0 + warp * U;
+    TileWalk<D, U> walk(p, pc.b, kv_head, issue, lane);
+    walk.fetch(pc.t1 - issue);
     auto copy_next = [&](uint32_t into) {
       if (issue < pc.t1) {
-        walk.template load<true>(into, place.cp, lane);
-        issue += kWarps;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (issue + u < pc.t1) walk.template load<true>(u, into + u * R::kStageBytes, place.cp, lane);
+        issue += U * kWarps;
         walk.advance();
-        if (issue < pc.t1) walk.fetch();
+        walk.fetch(pc.t1 - issue);
       }
       cp_commit();
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * R::kStageBytes);
+    for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * kStep);
     stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
     check_blocks(p, pc.b, pc.t0, pc.t1);
     __syncthreads();
@@ -665,25 +712,26 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
 
     Acc<D, NT> acc;
     acc.clear();
-    constexpr uint32_t kLast = (kStages - 1) * R::kStageBytes;
+    constexpr uint32_t kLast = (kStages - 1) * kStep;
     uint32_t st = base, into = base + kLast;
-    for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
+    for (int tile = pc.t0 + warp * U; tile < pc.t1; tile += U * kWarps) {
       cp_wait<kStages - 2>();
       __syncwarp();
-      copy_next(into);  // into the stage that the previous tile has left
-      const int left = n - tile * kTile;
-      if (left >= kTile)
-        take_tile<T, D, NT, false>(acc, q, st, place, codes, p.shl16, left, lane);
+      copy_next(into);  // into the stage that the previous step has left
+      // a piece that ends before its sequence may end inside a step
+      const int left = min(n, pc.t1 * kTile) - tile * kTile;
+      if (left >= U * kTile)
+        take_tiles<T, D, NT, false>(acc, q, st, place, codes, p.shl16, left, lane);
       else
-        take_tile<T, D, NT, true>(acc, q, st, place, codes, p.shl16, left, lane);
+        take_tiles<T, D, NT, true>(acc, q, st, place, codes, p.shl16, left, lane);
       into = st;
-      st = st == base + kLast ? base : st + R::kStageBytes;
+      st = st == base + kLast ? base : st + kStep;
       __syncwarp();  // every lane is done with this stage before it is refilled
     }
     cp_wait<0>();
     __syncthreads();  // the ring is free: it takes the warps' results
 
-    const int nact = min(kWarps, pc.t1 - pc.t0);
+    const int nact = min(kWarps, (pc.t1 - pc.t0 + U - 1) / U);
     float* red = reinterpret_cast<float*>(smem);
     if (warp < nact) {
 #pragma unroll
@@ -816,21 +864,21 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
     const int h_in = pc.hv % p.chunks * H;
     const int heads = min(H, group - h_in);
     const int head0 = kv_head * group + h_in;
-    const uint32_t base = smem_u32(smem) + warp * kStages * R::kHalf;
+    const uint32_t base = smem_u32(smem) + warp * kScoreStages * R::kHalf;
     int issue = pc.t0 + warp;
-    TileWalk<D> walk(p, pc.b, kv_head, issue, lane);
-    if (issue < pc.t1) walk.fetch();
+    TileWalk<D, 1> walk(p, pc.b, kv_head, issue, lane);
+    walk.fetch(pc.t1 - issue);
     auto copy_next = [&](uint32_t into) {
       if (issue < pc.t1) {
-        walk.template load<false>(into, place.cp, lane);
+        walk.template load<false>(0, into, place.cp, lane);
         issue += kWarps;
         walk.advance();
-        if (issue < pc.t1) walk.fetch();
+        walk.fetch(pc.t1 - issue);
       }
       cp_commit();
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * R::kHalf);
+    for (int s = 0; s < kScoreStages - 1; ++s) copy_next(base + s * R::kHalf);
     stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
     __syncthreads();
     Query<T, D, NT> q;
@@ -844,13 +892,13 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
         lse[t][e] = h < heads ? p.lse[(int64_t)pc.b * p.heads + head0 + h] * 1.4426950408889634f : INFINITY;
       }
     // a second walk, for the scores' addresses
-    TileWalk<D> to(p, pc.b, kv_head, pc.t0 + warp, lane);
+    TileWalk<D, 1> to(p, pc.b, kv_head, pc.t0 + warp, lane);
     float* const scores = p.scores + (size_t)kv_head * p.block_size;
-    constexpr uint32_t kLast = (kStages - 1) * R::kHalf;
+    constexpr uint32_t kLast = (kScoreStages - 1) * R::kHalf;
     uint32_t st = base, into = base + kLast;
     for (int tile = pc.t0 + warp; tile < pc.t1; tile += kWarps) {
-      to.fetch();
-      cp_wait<kStages - 2>();
+      to.fetch(1);
+      cp_wait<kScoreStages - 2>();
       __syncwarp();
       copy_next(into);
       float s[NT][4];
@@ -871,7 +919,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
       if (c < 2) {
         const int r = r0 + c * 8;
         if (tile * kTile + r < n)
-          atomicAdd(scores + (size_t)to.blk * ((uint32_t)p.kv_heads * p.block_size) + to.in * kTile + r,
+          atomicAdd(scores + (size_t)to.blk[0] * ((uint32_t)p.kv_heads * p.block_size) + to.in * kTile + r,
                     c == 0 ? w0 : w1);
       }
       to.advance();
@@ -885,7 +933,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
 template <typename T, int D, int NT>
 cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
   constexpr int H = NT * 8;
-  constexpr int ring = kWarps * kStages * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
+  constexpr int ring = kWarps * kStages * kTiles<D, NT> * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
   p.ring_bytes = ring > red ? ring : red;
   const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.direct ? 0 : (p.batch + 1) * 4);
   static PerDeviceOnce attr;
@@ -905,7 +953,7 @@ cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
 template <typename T, int D, int NT>
 cudaError_t launch_score(Kv4DecodeParams p, cudaStream_t s) {
   constexpr int H = NT * 8;
-  p.ring_bytes = kWarps * kStages * Ring<D>::kHalf;
+  p.ring_bytes = kWarps * kScoreStages * Ring<D>::kHalf;
   const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.batch + 1) * 4;
   static PerDeviceOnce attr;
   cudaError_t e = attr.run([&] {
@@ -953,7 +1001,7 @@ Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len
   const int64_t items = (int64_t)batch * kv_heads * plan.chunks;
   constexpr int kDirectTiles = 32;
   plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
-  const int resident = dim * plan.head_tiles <= 128 ? RES : 2;  // kResident
+  const int resident = dim * plan.head_tiles <= 128 ? 3 : 2;  // kResident
   plan.ctas = plan.direct ? (int)items : resident * device_sm_count();
   plan.max_batch = kv4::kMaxBatch;
   return plan;
