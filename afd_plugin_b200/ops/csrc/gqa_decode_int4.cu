@@ -776,14 +776,18 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   }
 }
 
-// Joins the partials of every (sequence, head) that more than one CTA worked
-// on, and writes the empty sequences.  One block per (sequence, query head).
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, int heads_chunk, int ctas) {
-  __shared__ int s_sum[2][4];
-  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+// Joins the partials of every (sequence, head chunk) that more than one CTA
+// worked on, and writes the empty sequences.  One block per (sequence, head
+// chunk); a thread holds 4 dims of one head.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) join_kernel(Kv4DecodeParams p) {
+  constexpr int H = NT * 8;
+  __shared__ int s_sum[2][8];
+  const int heads_v = p.kv_heads * p.chunks;
+  const int b = blockIdx.x / heads_v, hv = blockIdx.x % heads_v;
+  const int tiles = tiles_of(seq_len_of(p, b));
   int before = 0, all = 0;
-  for (int i = threadIdx.x; i < p.batch; i += blockDim.x) {
+  for (int i = threadIdx.x; i < p.batch; i += 256) {
     const int t = cost_of(tiles_of(seq_len_of(p, i)));
     all += t;
     if (i < b) before += t;
@@ -798,40 +802,52 @@ __global__ void __launch_bounds__(128) join_kernel(Kv4DecodeParams p, int dim, i
     s_sum[1][threadIdx.x / 32] = all;
   }
   __syncthreads();
-  before = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
-  all = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
-  const int tiles = tiles_of(seq_len_of(p, b));
-  T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head) * dim;
-  pdl_wait();
-  if (tiles == 0) {
-    for (int d = threadIdx.x; d < dim; d += blockDim.x) out[d] = from_f32<T>(0.f);
-    if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = -INFINITY;
-    return;
+  before = all = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += s_sum[0][w];
+    all += s_sum[1][w];
   }
   const int group = p.heads / p.kv_heads;
-  const int kv_head = head / group, hc = head % group / heads_chunk, h = head % group % heads_chunk;
-  const int heads_v = p.kv_heads * p.chunks;
-  const int64_t share = share_of((int64_t)all * heads_v, ctas);
-  const int64_t start = (int64_t)before * heads_v + (int64_t)(kv_head * p.chunks + hc) * cost_of(tiles) + kPieceCost;
+  const int h_in = hv % p.chunks * H, head0 = hv / p.chunks * group + h_in, heads = min(H, group - h_in);
+  T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head0) * D;
+  float* lse = p.lse == nullptr ? nullptr : p.lse + (int64_t)b * p.heads + head0;
+  const int64_t share = share_of((int64_t)all * heads_v, p.ctas);
+  const int64_t start = (int64_t)before * heads_v + (int64_t)hv * cost_of(tiles) + kPieceCost;
   const int64_t c0 = start / share, c1 = (start + tiles - 1) / share;
-  if (c0 == c1) return;  // one CTA had all of it and wrote the result
-  auto slot = [&](int64_t c) { return (2 * c + (c == c0 ? 1 : 0)) * heads_chunk + h; };
-  float m = kLowest;
-  for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, p.part_ml[slot(c) * 2]);
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  const int d0 = threadIdx.x, d1 = threadIdx.x + 128;
+  pdl_wait();
+  if (tiles > 0 && c0 == c1) return;  // one CTA had all of it and wrote the result
+  for (int i = threadIdx.x; i < heads * (D / 4); i += 256) {
+    const int h = i / (D / 4), d4 = i % (D / 4) * 4;
+    float m = kLowest, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (tiles > 0) {
+      const int n = (int)(c1 - c0) + 1;
+      // piece k's slot: the first begins with the first tile, the others begin shares
+      auto slot = [&](int k) { return (2 * (c0 + k) + (k == 0 ? 1 : 0)) * H + h; };
 #pragma unroll 4
-  for (int64_t c = c0; c <= c1; ++c) {
-    const int64_t sl = slot(c);
-    const float f = fast_exp2(p.part_ml[sl * 2] - m);
-    l = fmaf(p.part_ml[sl * 2 + 1], f, l);
-    if (d0 < dim) o0 = fmaf(p.part_o[sl * dim + d0], f, o0);
-    if (d1 < dim) o1 = fmaf(p.part_o[sl * dim + d1], f, o1);
+      for (int k = 0; k < n; ++k) m = fmaxf(m, p.part_ml[slot(k) * 2]);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const int64_t sl = slot(k);
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + sl * 2);
+        const float4 v = *reinterpret_cast<const float4*>(p.part_o + sl * D + d4);
+        const float f = fast_exp2(ml.x - m);
+        l = fmaf(ml.y, f, l);
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* to = out + h * D + d4;
+    to[0] = from_f32<T>(o.x * inv);
+    to[1] = from_f32<T>(o.y * inv);
+    to[2] = from_f32<T>(o.z * inv);
+    to[3] = from_f32<T>(o.w * inv);
+    if (d4 == 0 && lse != nullptr) lse[h] = (m + log2f(l)) * 0.6931471805599453f;
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (d0 < dim) out[d0] = from_f32<T>(o0 * inv);
-  if (d1 < dim) out[d1] = from_f32<T>(o1 * inv);
-  if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // Adds every position's probability to its score.  The same shares of tiles;
@@ -944,7 +960,7 @@ cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   decode_kernel<T, D, NT><<<p.ctas, kDecThreads, smem, s>>>(p);
   if (!p.direct) {
-    e = launch_pdl(join_kernel<T>, dim3((unsigned)(p.batch * p.heads)), dim3(128), 0, s, p, D, H, p.ctas);
+    e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)(p.batch * p.kv_heads * p.chunks)), dim3(256), 0, s, p);
     if (e != cudaSuccess) return e;
   }
   return cudaGetLastError();

@@ -352,7 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             for (int j = 0; j < 32; ++j) v[j] = 0;
           }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part[(c0 + j) * kBM + quarter * 32 + lane] = v[j];
+          for (int j = 0; j < 32; ++j)
+            if (row < a.t) part[(c0 + j) * kBM + quarter * 32 + lane] = v[j];
         }
       } else {
 #pragma unroll 1
@@ -371,34 +372,35 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     cluster.sync();
     int m, n;
     tile_at(a, first, m, n);
-    // 8 channels of one token per step: CTA r takes steps r, r + splits, ...
-    const int tok = threadIdx.x & 127;
-    if (threadIdx.x < 128 && m * kBM + tok < a.t) {
+    // Units of 8 channels of one token; CTA r takes channel octets r, r +
+    // splits, ..., its threads tokens innermost.
+    const int toks = min(kBM, a.t - m * kBM);
+    const int octets = (BN / 8 - split_rank + splits - 1) / splits;
+    for (int i = threadIdx.x; i < toks * octets; i += kThreads) {
+      const int tok = i % toks, c = (split_rank + i / toks * splits) * 8;
+      const int n0 = n * BN + c;
+      if (n0 >= a.n) continue;
+      int v[8] = {};
+      for (int r = 0; r < splits; ++r) {
+        const int* part = cluster.map_shared_rank(reinterpret_cast<int*>(sm.x[0]), r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += part[(c + j) * kBM + tok];
+      }
       const float xs = a.xs[m * kBM + tok];
-      for (int c = split_rank * 8; c < BN; c += splits * 8) {
-        int v[8] = {};
-        for (int r = 0; r < splits; ++r) {
-          const int* part = cluster.map_shared_rank(reinterpret_cast<int*>(sm.x[0]), r);
+      T* y = reinterpret_cast<T*>(a.y) + (int64_t)(m * kBM + tok) * a.n + n0;
+      if (a.out_vec && n0 + 8 <= a.n) {
+        constexpr int N = Vec16<T>::N;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += part[(c + j) * kBM + tok];
+        for (int u = 0; u < 8 / N; ++u) {
+          Vec16<T> o;
+#pragma unroll
+          for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>((float)v[u * N + j] * (xs * sm.ws[0][c + u * N + j]));
+          store16(y + u * N, o);
         }
-        const int n0 = n * BN + c;
-        T* y = reinterpret_cast<T*>(a.y) + (int64_t)(m * kBM + tok) * a.n + n0;
-        if (a.out_vec && n0 + 8 <= a.n) {
-          constexpr int N = Vec16<T>::N;
+      } else {
 #pragma unroll
-          for (int u = 0; u < 8 / N; ++u) {
-            Vec16<T> o;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-              o.v[j] = from_f32<T>((float)v[u * N + j] * (xs * sm.ws[0][c + u * N + j]));
-            store16(y + u * N, o);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n0 + j < a.n) y[j] = from_f32<T>((float)v[j] * (xs * sm.ws[0][c + j]));
-        }
+        for (int j = 0; j < 8; ++j)
+          if (n0 + j < a.n) y[j] = from_f32<T>((float)v[j] * (xs * sm.ws[0][c + j]));
       }
     }
     cluster.sync();  // no CTA's shared memory goes away while another reads it

@@ -22,6 +22,7 @@
 // D = 128), and one read of the scores.  The cluster size spreads small
 // batches over the SMs.
 #include <cooperative_groups.h>
+#include <cstdlib>
 
 #include "device_state.h"
 #include "kv_int4.cuh"
@@ -268,9 +269,8 @@ cudaError_t launch_evict(Kv4EvictParams p, int cs, size_t smem, cudaStream_t s) 
 using namespace afd;
 
 int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s) {
-  // Small batches spread each (sequence, head) over up to 8 CTAs; two CTAs per SM are the aim.
-  int cs = 1;
-  while (cs < 8 && (int64_t)p.batch * p.kv_heads * cs * 2 <= 2 * device_sm_count()) cs *= 2;
+  const char* ev = getenv("KV4_CS");
+  const int cs = ev ? atoi(ev) : 8;
   const int per = (p.max_blocks * p.block_size + cs - 1) / cs;
   p.key_cap = per < 200 * 256 ? per : 200 * 256;
   const size_t smem = (size_t)p.key_cap * 4;

@@ -40,21 +40,41 @@ AFD_DEVICE void load8(float (&x)[8], const T* p, bool vec) {
   }
 }
 
-// grid.x covers (token, head, D / 8) and grid.y is 0 for K, 1 for V.  A thread's
-// 8 lanes of a group are neighbours and in range together (D % 64 == 0).
-template <typename T>
+// d / s, correctly rounded, with r the correctly rounded 1 / s: a quotient
+// within an ulp and one exact remainder (Markstein 1990).  Holds because s has
+// 8 significant bits (its mantissa is not all ones) and both are far from the
+// ends of the exponent range.
+AFD_DEVICE float quotient(float d, float s, float r) {
+  const float q = d * r;
+  return fmaf(fmaf(-q, s, d), r, q);
+}
+
+// Block and offset of a slot; a power-of-two block size is a shift.
+AFD_DEVICE void split_slot(int64_t slot, int block_size, int shift, int64_t& blk, int& off) {
+  if (shift >= 0) {
+    blk = slot >> shift;
+    off = (int)slot & (block_size - 1);
+  } else {
+    blk = slot / block_size;
+    off = (int)(slot - blk * block_size);
+  }
+}
+
+// A block takes kThreads / parts rows (token, head); grid.y is 0 for K, 1 for V.
+// D / 8 lanes hold a row, so the 8 lanes of a group are neighbours.
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
-  const int parts = p.dim / 8;
-  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const bool live = idx < (int64_t)p.tokens * p.kv_heads * parts;
-  const int64_t at = live ? idx : 0;
-  const int part = (int)(at % parts);
-  const int64_t row = at / parts;
-  const int head = (int)(row % p.kv_heads);
-  const int64_t tok = row / p.kv_heads;
+  constexpr int kParts = D / 8, kRows = kThreads / kParts;
+  const int part = threadIdx.x % kParts;
+  const int64_t rows = (int64_t)p.tokens * p.kv_heads;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kParts;
+  const bool live = row < rows;
+  const uint32_t tok = (uint32_t)(live ? row / (uint32_t)p.kv_heads : 0);
+  const uint32_t head = live ? (uint32_t)(row - (int64_t)tok * p.kv_heads) : 0;
   const bool is_v = blockIdx.y != 0;
   const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + tok * (is_v ? p.v_st : p.k_st) +
                  head * (is_v ? p.v_sh : p.k_sh) + part * 8;
+  const int64_t slot = p.slots[tok];
   float x[8];
   load8(x, src, p.vec != 0);
   float lo = x[0], hi = x[0];
@@ -69,7 +89,6 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   if (!live) return;
-  const int64_t slot = p.slots[tok];
   if (slot < 0 || slot >= p.num_slots) {
     if (part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
     return;
@@ -77,39 +96,52 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
   const float zero = bf16_down(lo);
   const float step = bf16_up_nonneg(__fdiv_rn(hi - zero, 15.f));
   uint32_t word = 0;
+  if (step > 1e-25f && step < 1e25f) {
+    const float r = __frcp_rn(step);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = step > 0.f ? rintf(__fdiv_rn(x[i] - zero, step)) : 0.f;
-    word |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      // adding 1.5 * 2^23 rounds to a whole number, ties to even, in the low bits
+      const float c = fminf(fmaxf(quotient(x[i] - zero, step, r), 0.f), 15.f) + 12582912.f;
+      word |= (__float_as_uint(c) & 15u) << (4 * i);
+    }
+  } else if (step > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - zero, step)), 0.f), 15.f) << (4 * i);
   }
-  const int64_t blk = slot / p.block_size, off = slot % p.block_size;
+  int64_t blk;
+  int off;
+  split_slot(slot, p.block_size, p.block_shift, blk, off);
   const int64_t dst = (blk * p.kv_heads + head) * p.block_size + off;
   uint8_t* codes = is_v ? p.v_codes : p.k_codes;
   uint32_t* scale = is_v ? p.v_scale : p.k_scale;
-  reinterpret_cast<uint32_t*>(codes + dst * (p.dim / 2))[part] = word;
+  reinterpret_cast<uint32_t*>(codes + dst * (D / 2))[part] = word;
   if (part % 8 == 0)
-    scale[dst * (p.dim / kGroup) + part / 8] = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
+    scale[dst * (D / kGroup) + part / 8] = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
   if (p.scores != nullptr && !is_v && part == 0) p.scores[dst] = 0.f;
 }
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv4ReadParams p) {
-  const int parts = p.dim / 8;
-  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (idx >= (int64_t)p.tokens * p.kv_heads * parts) return;
-  const int part = (int)(idx % parts);
-  const int64_t row = idx / parts;
-  const int head = (int)(row % p.kv_heads);
-  const int64_t slot = p.slots[row / p.kv_heads];
+  constexpr int kParts = D / 8, kRows = kThreads / kParts;
+  const int part = threadIdx.x % kParts;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kParts;
+  if (row >= (int64_t)p.tokens * p.kv_heads) return;
+  const uint32_t tok = (uint32_t)(row / (uint32_t)p.kv_heads);
+  const uint32_t head = (uint32_t)(row - (int64_t)tok * p.kv_heads);
+  const int64_t slot = p.slots[tok];
   const bool is_v = blockIdx.y != 0;
-  T* dst = reinterpret_cast<T*>(is_v ? p.v : p.k) + idx * 8;
+  T* dst = reinterpret_cast<T*>(is_v ? p.v : p.k) + row * D + part * 8;
   float x[8] = {};
   if (slot < 0 || slot >= p.num_slots) {
     if (part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
   } else {
-    const int64_t src = (slot / p.block_size * p.kv_heads + head) * p.block_size + slot % p.block_size;
-    const uint32_t word = reinterpret_cast<const uint32_t*>((is_v ? p.v_codes : p.k_codes) + src * (p.dim / 2))[part];
-    const uint32_t pair = (is_v ? p.v_scale : p.k_scale)[src * (p.dim / kGroup) + part / 8];
+    int64_t blk;
+    int off;
+    split_slot(slot, p.block_size, p.block_shift, blk, off);
+    const int64_t src = (blk * p.kv_heads + head) * p.block_size + off;
+    const uint32_t word = reinterpret_cast<const uint32_t*>((is_v ? p.v_codes : p.k_codes) + src * (D / 2))[part];
+    const uint32_t pair = (is_v ? p.v_scale : p.k_scale)[src * (D / kGroup) + part / 8];
     const float step = pair_step(pair), zero = pair_zero(pair);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word >> (4 * i)) & 15u), step, zero);
@@ -124,27 +156,51 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv4ReadParams p) {
   }
 }
 
+// Rows (token, head) a block covers, and the grid for all of them.
+template <int D> dim3 row_grid(int64_t rows) {
+  constexpr int kRows = kThreads / (D / 8);
+  return dim3((unsigned)((rows + kRows - 1) / kRows), 2);
+}
+int shift_of(int block_size) { return (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1; }
+
+template <typename T>
+void write(Kv4WriteParams p, cudaStream_t s) {
+  const int64_t rows = (int64_t)p.tokens * p.kv_heads;
+  p.block_shift = shift_of(p.block_size);
+  switch (p.dim) {
+    case 64: write_kernel<T, 64><<<row_grid<64>(rows), kThreads, 0, s>>>(p); break;
+    case 128: write_kernel<T, 128><<<row_grid<128>(rows), kThreads, 0, s>>>(p); break;
+    default: write_kernel<T, 256><<<row_grid<256>(rows), kThreads, 0, s>>>(p);
+  }
+}
+template <typename T>
+void read(Kv4ReadParams p, cudaStream_t s) {
+  const int64_t rows = (int64_t)p.tokens * p.kv_heads;
+  p.block_shift = shift_of(p.block_size);
+  switch (p.dim) {
+    case 64: read_kernel<T, 64><<<row_grid<64>(rows), kThreads, 0, s>>>(p); break;
+    case 128: read_kernel<T, 128><<<row_grid<128>(rows), kThreads, 0, s>>>(p); break;
+    default: read_kernel<T, 256><<<row_grid<256>(rows), kThreads, 0, s>>>(p);
+  }
+}
+
 }  // namespace kv4
 }  // namespace afd
 
 using namespace afd;
 
 void launch_kv4_write(const Kv4WriteParams& p, int dtype, cudaStream_t s) {
-  const int64_t n = (int64_t)p.tokens * p.kv_heads * (p.dim / 8);
-  const dim3 grid((unsigned)((n + kv4::kThreads - 1) / kv4::kThreads), 2);
   switch (dtype) {
-    case kF32: kv4::write_kernel<float><<<grid, kv4::kThreads, 0, s>>>(p); break;
-    case kF16: kv4::write_kernel<__half><<<grid, kv4::kThreads, 0, s>>>(p); break;
-    default: kv4::write_kernel<__nv_bfloat16><<<grid, kv4::kThreads, 0, s>>>(p); break;
+    case kF32: kv4::write<float>(p, s); break;
+    case kF16: kv4::write<__half>(p, s); break;
+    default: kv4::write<__nv_bfloat16>(p, s); break;
   }
 }
 
 void launch_kv4_read(const Kv4ReadParams& p, int dtype, cudaStream_t s) {
-  const int64_t n = (int64_t)p.tokens * p.kv_heads * (p.dim / 8);
-  const dim3 grid((unsigned)((n + kv4::kThreads - 1) / kv4::kThreads), 2);
   switch (dtype) {
-    case kF32: kv4::read_kernel<float><<<grid, kv4::kThreads, 0, s>>>(p); break;
-    case kF16: kv4::read_kernel<__half><<<grid, kv4::kThreads, 0, s>>>(p); break;
-    default: kv4::read_kernel<__nv_bfloat16><<<grid, kv4::kThreads, 0, s>>>(p); break;
+    case kF32: kv4::read<float>(p, s); break;
+    case kF16: kv4::read<__half>(p, s); break;
+    default: kv4::read<__nv_bfloat16>(p, s); break;
   }
 }

@@ -375,6 +375,7 @@ struct Kv4WriteParams {
   int64_t num_slots;
   int tokens, kv_heads, dim, block_size;
   int vec;                    // rows are 16-byte aligned
+  int block_shift;            // set by the launcher
 };
 struct Kv4ReadParams {
   void *k, *v;                // [tokens, kv_heads, dim]
@@ -384,6 +385,7 @@ struct Kv4ReadParams {
   int* status;
   int64_t num_slots;
   int tokens, kv_heads, dim, block_size;
+  int block_shift;            // set by the launcher
 };
 void launch_kv4_write(const Kv4WriteParams& p, int dtype, cudaStream_t s);
 void launch_kv4_read(const Kv4ReadParams& p, int dtype, cudaStream_t s);
