@@ -534,7 +534,7 @@ void gqa_cache_write_int4(at::Tensor& kc, at::Tensor& ks, at::Tensor& vc, at::Te
   check_same_device(slots, kc, op, "slot_mapping");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
                   slots.size(0) == k.size(0), op, ": int64 slot_mapping [tokens]");
-  TORCH_CHECK(k.size(0) <= INT32_MAX, op, ": at most 2^31 - 1 tokens");
+  TORCH_CHECK(k.size(0) * sh.kv_heads <= INT32_MAX, op, ": at most 2^31 - 1 rows");
   Kv4WriteParams p{};
   p.scores = check_kv4_scores(scores, kc, op);
   if (k.size(0) == 0) return;
@@ -573,7 +573,7 @@ std::tuple<at::Tensor, at::Tensor> gqa_cache_read_int4(const at::Tensor& kc, con
   const Kv4Shape sh = check_kv4(kc, ks, vc, vs, op);
   check_same_device(slots, kc, op, "slots");
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
-                  slots.size(0) <= INT32_MAX, op, ": int64 slots [tokens]");
+                  slots.size(0) * sh.kv_heads <= INT32_MAX, op, ": int64 slots [tokens], at most 2^31 - 1 rows");
   c10::cuda::CUDAGuard g(kc.device());
   const int64_t n = slots.size(0);
   auto k = at::empty({n, sh.kv_heads, sh.dim}, kc.options().dtype(dtype));

@@ -776,18 +776,22 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   }
 }
 
-// Joins the partials of every (sequence, head chunk) that more than one CTA
-// worked on, and writes the empty sequences.  One block per (sequence, head
-// chunk); a thread holds 4 dims of one head.
+// Joins the partials of every (sequence, head) that more than one CTA worked
+// on, and writes the empty sequences.  One block per (sequence, query head):
+// its warps take the pieces in turn, and merge through shared memory.
+constexpr int kJoinWarps = 8;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) join_kernel(Kv4DecodeParams p) {
-  constexpr int H = NT * 8;
-  __shared__ int s_sum[2][8];
-  const int heads_v = p.kv_heads * p.chunks;
-  const int b = blockIdx.x / heads_v, hv = blockIdx.x % heads_v;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Kv4DecodeParams p) {
+  constexpr int H = NT * 8, kThreads = kJoinWarps * 32, V = D / 32;  // dims a lane holds
+  __shared__ int s_sum[2][kJoinWarps];
+  __shared__ float s_ml[2][kJoinWarps], s_o[kJoinWarps][D];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int heads_v = p.kv_heads * p.chunks, group = p.heads / p.kv_heads;
+  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+  const int hv = head / group * p.chunks + head % group / H, h = head % group % H;
   const int tiles = tiles_of(seq_len_of(p, b));
   int before = 0, all = 0;
-  for (int i = threadIdx.x; i < p.batch; i += 256) {
+  for (int i = threadIdx.x; i < p.batch; i += kThreads) {
     const int t = cost_of(tiles_of(seq_len_of(p, i)));
     all += t;
     if (i < b) before += t;
@@ -797,56 +801,60 @@ __global__ void __launch_bounds__(256) join_kernel(Kv4DecodeParams p) {
     before += __shfl_xor_sync(0xffffffffu, before, o);
     all += __shfl_xor_sync(0xffffffffu, all, o);
   }
-  if ((threadIdx.x & 31) == 0) {
-    s_sum[0][threadIdx.x / 32] = before;
-    s_sum[1][threadIdx.x / 32] = all;
+  if (lane == 0) {
+    s_sum[0][warp] = before;
+    s_sum[1][warp] = all;
   }
   __syncthreads();
   before = all = 0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < kJoinWarps; ++w) {
     before += s_sum[0][w];
     all += s_sum[1][w];
   }
-  const int group = p.heads / p.kv_heads;
-  const int h_in = hv % p.chunks * H, head0 = hv / p.chunks * group + h_in, heads = min(H, group - h_in);
-  T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head0) * D;
-  float* lse = p.lse == nullptr ? nullptr : p.lse + (int64_t)b * p.heads + head0;
   const int64_t share = share_of((int64_t)all * heads_v, p.ctas);
   const int64_t start = (int64_t)before * heads_v + (int64_t)hv * cost_of(tiles) + kPieceCost;
-  const int64_t c0 = start / share, c1 = (start + tiles - 1) / share;
+  const int64_t c0 = start / share;
+  const int n = tiles > 0 ? (int)((start + tiles - 1) / share - c0) + 1 : 0;
   pdl_wait();
-  if (tiles > 0 && c0 == c1) return;  // one CTA had all of it and wrote the result
-  for (int i = threadIdx.x; i < heads * (D / 4); i += 256) {
-    const int h = i / (D / 4), d4 = i % (D / 4) * 4;
-    float m = kLowest, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (tiles > 0) {
-      const int n = (int)(c1 - c0) + 1;
-      // piece k's slot: the first begins with the first tile, the others begin shares
-      auto slot = [&](int k) { return (2 * (c0 + k) + (k == 0 ? 1 : 0)) * H + h; };
+  if (n == 1) return;  // one CTA had all of it and wrote the result
+  float m = kLowest, l = 0.f, o[V] = {};
 #pragma unroll 4
-      for (int k = 0; k < n; ++k) m = fmaxf(m, p.part_ml[slot(k) * 2]);
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const int64_t sl = slot(k);
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + sl * 2);
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + sl * D + d4);
-        const float f = fast_exp2(ml.x - m);
-        l = fmaf(ml.y, f, l);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
-      }
+  for (int k = warp; k < n; k += kJoinWarps) {
+    // piece k's slot: the first begins with the first tile, the others begin shares
+    const int64_t slot = (2 * (c0 + k) + (k == 0 ? 1 : 0)) * H + h;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = p.part_o[slot * D + i * 32 + lane];
+    const float mx = fmaxf(m, ml.x), f = fast_exp2(m - mx), g = fast_exp2(ml.x - mx);
+    m = mx;
+    l = l * f + ml.y * g;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = o[i] * f + v[i] * g;
+  }
+  if (lane == 0) {
+    s_ml[0][warp] = m;
+    s_ml[1][warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) s_o[warp][i * 32 + lane] = o[i];
+  __syncthreads();
+  m = kLowest;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, s_ml[0][w]);
+  for (int d = threadIdx.x; d < D; d += kThreads) {
+    l = 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float f = fast_exp2(s_ml[0][w] - m);
+      l = fmaf(s_ml[1][w], f, l);
+      sum = fmaf(s_o[w][d], f, sum);
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    T* to = out + h * D + d4;
-    to[0] = from_f32<T>(o.x * inv);
-    to[1] = from_f32<T>(o.y * inv);
-    to[2] = from_f32<T>(o.z * inv);
-    to[3] = from_f32<T>(o.w * inv);
-    if (d4 == 0 && lse != nullptr) lse[h] = (m + log2f(l)) * 0.6931471805599453f;
+    reinterpret_cast<T*>(p.out)[((int64_t)b * p.heads + head) * D + d] = from_f32<T>(sum * inv);
+    if (d == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = (m + log2f(l)) * 0.6931471805599453f;
   }
 }
 
@@ -960,7 +968,7 @@ cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   decode_kernel<T, D, NT><<<p.ctas, kDecThreads, smem, s>>>(p);
   if (!p.direct) {
-    e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)(p.batch * p.kv_heads * p.chunks)), dim3(256), 0, s, p);
+    e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)(p.batch * p.heads)), dim3(kJoinWarps * 32), 0, s, p);
     if (e != cudaSuccess) return e;
   }
   return cudaGetLastError();

@@ -475,7 +475,7 @@ cudaError_t run(const Int8GemmParams& p, cudaStream_t s) {
   int splits = sms / tiles;
   if (splits > 8) splits = 8;
   if (splits > a.k_blocks / 4) splits = a.k_blocks / 4;
-  if (splits > 1) return launch<T, 128, 4, true>(p, a, splits, s);
+  if (splits > 1) return launch<T, 128, 6, true>(p, a, splits, s);
   return launch<T, 128, 6, false>(p, a, 1, s);
 }
 

@@ -52,7 +52,7 @@ struct EvictView {
         block_rows((int64_t)q.kv_heads * q.block_size) {}
   // Cache row of a position.  A block id outside the pool is reported and replaced by the padding block.
   AFD_DEVICE int64_t row(int pos) const {
-    const int pg = pos / p.block_size;
+    const int pg = p.block_shift >= 0 ? pos >> p.block_shift : pos / p.block_size;
     int blk = table[pg];
     if ((unsigned)blk >= (unsigned)p.num_blocks) {
       if (p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   __shared__ int s_warp[2][kEvWarps];         // kept-for-sure / tied positions of each warp's run
   __shared__ int s_cta[2];                    // the CTA's totals, read by the others
   __shared__ uint32_t s_scan[8];
+  __shared__ int64_t s_rows[2][2][kRows];     // source and destination rows of this chunk and the next
 
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -205,7 +206,9 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   for (int i = rank * kEvThreads + tid; i < p.recent; i += cs * kEvThreads) kept[need + i] = m + i;
   cluster.sync();  // the list is complete, and visible to the cluster
 
-  // Move.  16-byte units of codes and 4-byte words of pairs and scores.
+  // Move.  16-byte units of codes and 4-byte words of pairs and scores.  Each
+  // row's source and destination are looked up once, by one thread, a chunk
+  // ahead of their use.
   uint4* const kc = reinterpret_cast<uint4*>(p.k_codes);
   uint4* const vc = reinterpret_cast<uint4*>(p.v_codes);
   auto unit = [&](int64_t row, int u) {
@@ -215,30 +218,39 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
     return w < G ? p.k_scale + row * G + w
                  : (w < 2 * G ? p.v_scale + row * G + (w - G) : reinterpret_cast<uint32_t*>(p.scores) + row);
   };
-  const int step = cs * kRows;
-  for (int r0 = rank * kRows; r0 - rank * kRows < p.budget; r0 += step) {
+  const int step = cs * kRows, skip = rank * kRows;
+  const bool is_dst = tid >= kEvThreads / 2;
+  auto look_up = [&](int buf, int r0) {  // rows r0 .. r0 + kRows - 1
+    for (int r = tid & (kEvThreads / 2 - 1); r < kRows; r += kEvThreads / 2)
+      if (r0 + r < p.budget) s_rows[buf][is_dst][r] = view.row(is_dst ? r0 + r : kept[r0 + r]);
+  };
+  look_up(0, skip);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = skip; r0 - skip < p.budget; r0 += step, buf ^= 1) {
     uint4 x[kUnits];
     uint32_t y[kWords];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int j = k * kEvThreads + tid, r = r0 + j / kRowUnits;
-      if (r < p.budget) x[k] = *unit(view.row(kept[r]), j % kRowUnits);
+      const int j = k * kEvThreads + tid, r = j / kRowUnits;
+      if (r0 + r < p.budget) x[k] = *unit(s_rows[buf][0][r], j % kRowUnits);
     }
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-      const int j = k * kEvThreads + tid, r = r0 + j / kRowWords;
-      if (j < kRows * kRowWords && r < p.budget) y[k] = *word(view.row(kept[r]), j % kRowWords);
+      const int j = k * kEvThreads + tid, r = j / kRowWords;
+      if (j < kRows * kRowWords && r0 + r < p.budget) y[k] = *word(s_rows[buf][0][r], j % kRowWords);
     }
+    look_up(buf ^ 1, r0 + step);
     cluster.sync();
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int j = k * kEvThreads + tid, r = r0 + j / kRowUnits;
-      if (r < p.budget) *unit(view.row(r), j % kRowUnits) = x[k];
+      const int j = k * kEvThreads + tid, r = j / kRowUnits;
+      if (r0 + r < p.budget) *unit(s_rows[buf][1][r], j % kRowUnits) = x[k];
     }
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
-      const int j = k * kEvThreads + tid, r = r0 + j / kRowWords;
-      if (j < kRows * kRowWords && r < p.budget) *word(view.row(r), j % kRowWords) = y[k];
+      const int j = k * kEvThreads + tid, r = j / kRowWords;
+      if (j < kRows * kRowWords && r0 + r < p.budget) *word(s_rows[buf][1][r], j % kRowWords) = y[k];
     }
   }
 }
@@ -247,7 +259,7 @@ template <int D>
 cudaError_t launch_evict(Kv4EvictParams p, int cs, size_t smem, cudaStream_t s) {
   static PerDeviceOnce attr;
   cudaError_t e =
-      attr.run([&] { return cudaFuncSetAttribute(evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
+      attr.run([&] { return cudaFuncSetAttribute(evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 46080 * 4); });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.batch * p.kv_heads * cs));
@@ -272,7 +284,8 @@ int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s) {
   const char* ev = getenv("KV4_CS");
   const int cs = ev ? atoi(ev) : 8;
   const int per = (p.max_blocks * p.block_size + cs - 1) / cs;
-  p.key_cap = per < 200 * 256 ? per : 200 * 256;
+  p.block_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(p.block_size) : -1;
+  p.key_cap = per < 46080 ? per : 46080;  // 180 KB
   const size_t smem = (size_t)p.key_cap * 4;
   switch (dim) {
     case 64: return (int)kv4::launch_evict<64>(p, cs, smem, s);

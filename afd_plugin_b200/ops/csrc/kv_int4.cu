@@ -49,8 +49,10 @@ AFD_DEVICE float quotient(float d, float s, float r) {
   return fmaf(fmaf(-q, s, d), r, q);
 }
 
-// Block and offset of a slot; a power-of-two block size is a shift.
-AFD_DEVICE void split_slot(int64_t slot, int block_size, int shift, int64_t& blk, int& off) {
+// Row (block, head, offset) of a slot in the cache; a power-of-two block size is a shift.
+AFD_DEVICE int64_t cache_row(int64_t slot, uint32_t head, int kv_heads, int block_size, int shift) {
+  int64_t blk;
+  int off;
   if (shift >= 0) {
     blk = slot >> shift;
     off = (int)slot & (block_size - 1);
@@ -58,25 +60,12 @@ AFD_DEVICE void split_slot(int64_t slot, int block_size, int shift, int64_t& blk
     blk = slot / block_size;
     off = (int)(slot - blk * block_size);
   }
+  return (blk * kv_heads + head) * block_size + off;
 }
 
-// A block takes kThreads / parts rows (token, head); grid.y is 0 for K, 1 for V.
-// D / 8 lanes hold a row, so the 8 lanes of a group are neighbours.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
-  constexpr int kParts = D / 8, kRows = kThreads / kParts;
-  const int part = threadIdx.x % kParts;
-  const int64_t rows = (int64_t)p.tokens * p.kv_heads;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kParts;
-  const bool live = row < rows;
-  const uint32_t tok = (uint32_t)(live ? row / (uint32_t)p.kv_heads : 0);
-  const uint32_t head = live ? (uint32_t)(row - (int64_t)tok * p.kv_heads) : 0;
-  const bool is_v = blockIdx.y != 0;
-  const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + tok * (is_v ? p.v_st : p.k_st) +
-                 head * (is_v ? p.v_sh : p.k_sh) + part * 8;
-  const int64_t slot = p.slots[tok];
-  float x[8];
-  load8(x, src, p.vec != 0);
+// Quantises the 8 values of this lane with the 64 of its 8 neighbours and
+// stores its word and, from the group's first lane, the (step, zero) pair.
+AFD_DEVICE void store_group(const float (&x)[8], bool live, uint32_t* word_at, uint32_t* pair_at, bool first) {
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
@@ -89,77 +78,93 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   if (!live) return;
-  if (slot < 0 || slot >= p.num_slots) {
-    if (part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
-    return;
-  }
   const float zero = bf16_down(lo);
   const float step = bf16_up_nonneg(__fdiv_rn(hi - zero, 15.f));
   uint32_t word = 0;
   if (step > 1e-25f && step < 1e25f) {
+    // Adding 1.5 * 2^23 rounds to a whole number, ties to even, in the low bits
+    // of 0x4B400000.  zero <= x and the step's rounding keep it in 0 .. 15.
     const float r = __frcp_rn(step);
+    constexpr uint32_t kOnes = 0x11111111u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // adding 1.5 * 2^23 rounds to a whole number, ties to even, in the low bits
-      const float c = fminf(fmaxf(quotient(x[i] - zero, step, r), 0.f), 15.f) + 12582912.f;
-      word |= (__float_as_uint(c) & 15u) << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i)
+      word += __float_as_uint(quotient(x[i] - zero, step, r) + 12582912.f) * (1u << (4 * i));
+    word -= 0x4B400000u * kOnes;
   } else if (step > 0.f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - zero, step)), 0.f), 15.f) << (4 * i);
   }
-  int64_t blk;
-  int off;
-  split_slot(slot, p.block_size, p.block_shift, blk, off);
-  const int64_t dst = (blk * p.kv_heads + head) * p.block_size + off;
-  uint8_t* codes = is_v ? p.v_codes : p.k_codes;
-  uint32_t* scale = is_v ? p.v_scale : p.k_scale;
-  reinterpret_cast<uint32_t*>(codes + dst * (D / 2))[part] = word;
-  if (part % 8 == 0)
-    scale[dst * (D / kGroup) + part / 8] = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
-  if (p.scores != nullptr && !is_v && part == 0) p.scores[dst] = 0.f;
+  *word_at = word;
+  if (first) *pair_at = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
+}
+
+// A block takes kThreads / parts rows (token, head), K and V of each.  D / 8
+// lanes hold a row, so the 8 lanes of a group are neighbours.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
+  constexpr int kParts = D / 8, kRows = kThreads / kParts;
+  const uint32_t part = threadIdx.x % kParts;
+  uint32_t row = blockIdx.x * kRows + threadIdx.x / kParts;
+  bool live = row < (uint32_t)p.tokens * (uint32_t)p.kv_heads;
+  row = live ? row : 0;
+  const uint32_t tok = row / (uint32_t)p.kv_heads, head = row - tok * (uint32_t)p.kv_heads;
+  const T* k = reinterpret_cast<const T*>(p.k) + (int64_t)tok * p.k_st + (int64_t)head * p.k_sh + part * 8;
+  const T* v = reinterpret_cast<const T*>(p.v) + (int64_t)tok * p.v_st + (int64_t)head * p.v_sh + part * 8;
+  const int64_t slot = p.slots[tok];
+  float x[8], y[8];
+  load8(x, k, p.vec != 0);
+  load8(y, v, p.vec != 0);
+  if (slot < 0 || slot >= p.num_slots) {
+    if (live && part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
+    live = false;
+  }
+  const int64_t dst = live ? cache_row(slot, head, p.kv_heads, p.block_size, p.block_shift) : 0;
+  const int64_t word = dst * kParts + part, pair = dst * (D / kGroup) + part / 8;
+  store_group(x, live, reinterpret_cast<uint32_t*>(p.k_codes) + word, p.k_scale + pair, part % 8 == 0);
+  store_group(y, live, reinterpret_cast<uint32_t*>(p.v_codes) + word, p.v_scale + pair, part % 8 == 0);
+  if (p.scores != nullptr && live && part == 0) p.scores[dst] = 0.f;
+}
+
+template <typename T>
+AFD_DEVICE void store_values(T* dst, uint32_t word, uint32_t pair) {
+  constexpr int N = Vec16<T>::N;
+  const float step = pair_step(pair), zero = pair_zero(pair);
+#pragma unroll
+  for (int u = 0; u < 8 / N; ++u) {
+    Vec16<T> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(fmaf((float)((word >> (4 * (u * N + i))) & 15u), step, zero));
+    store16(dst + u * N, v);
+  }
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv4ReadParams p) {
   constexpr int kParts = D / 8, kRows = kThreads / kParts;
-  const int part = threadIdx.x % kParts;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kParts;
-  if (row >= (int64_t)p.tokens * p.kv_heads) return;
-  const uint32_t tok = (uint32_t)(row / (uint32_t)p.kv_heads);
-  const uint32_t head = (uint32_t)(row - (int64_t)tok * p.kv_heads);
+  const uint32_t part = threadIdx.x % kParts;
+  const uint32_t row = blockIdx.x * kRows + threadIdx.x / kParts;
+  if (row >= (uint32_t)p.tokens * (uint32_t)p.kv_heads) return;
+  const uint32_t tok = row / (uint32_t)p.kv_heads, head = row - tok * (uint32_t)p.kv_heads;
   const int64_t slot = p.slots[tok];
-  const bool is_v = blockIdx.y != 0;
-  T* dst = reinterpret_cast<T*>(is_v ? p.v : p.k) + row * D + part * 8;
-  float x[8] = {};
+  uint32_t kw = 0, kp = 0, vw = 0, vp = 0;  // a zero step and zero: zeros
   if (slot < 0 || slot >= p.num_slots) {
     if (part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
   } else {
-    int64_t blk;
-    int off;
-    split_slot(slot, p.block_size, p.block_shift, blk, off);
-    const int64_t src = (blk * p.kv_heads + head) * p.block_size + off;
-    const uint32_t word = reinterpret_cast<const uint32_t*>((is_v ? p.v_codes : p.k_codes) + src * (D / 2))[part];
-    const uint32_t pair = (is_v ? p.v_scale : p.k_scale)[src * (D / kGroup) + part / 8];
-    const float step = pair_step(pair), zero = pair_zero(pair);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf((float)((word >> (4 * i)) & 15u), step, zero);
+    const int64_t src = cache_row(slot, head, p.kv_heads, p.block_size, p.block_shift);
+    kw = reinterpret_cast<const uint32_t*>(p.k_codes)[src * kParts + part];
+    vw = reinterpret_cast<const uint32_t*>(p.v_codes)[src * kParts + part];
+    kp = p.k_scale[src * (D / kGroup) + part / 8];
+    vp = p.v_scale[src * (D / kGroup) + part / 8];
   }
-  constexpr int N = Vec16<T>::N;
-#pragma unroll
-  for (int u = 0; u < 8 / N; ++u) {
-    Vec16<T> v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(x[u * N + i]);
-    store16(dst + u * N, v);
-  }
+  const int64_t at = (int64_t)row * D + part * 8;
+  store_values(reinterpret_cast<T*>(p.k) + at, kw, kp);
+  store_values(reinterpret_cast<T*>(p.v) + at, vw, vp);
 }
 
-// Rows (token, head) a block covers, and the grid for all of them.
 template <int D> dim3 row_grid(int64_t rows) {
   constexpr int kRows = kThreads / (D / 8);
-  return dim3((unsigned)((rows + kRows - 1) / kRows), 2);
+  return dim3((unsigned)((rows + kRows - 1) / kRows));
 }
 int shift_of(int block_size) { return (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1; }
 

@@ -435,7 +435,9 @@ struct Kv4EvictParams {
   int* status;                // or null
   int batch, kv_heads, block_size, num_blocks, max_blocks;
   int budget, recent;         // 0 <= recent <= budget, 1 <= budget
-  int key_cap;                // keys a CTA holds in shared memory; set by the launcher
+  // set by the launcher
+  int key_cap;                // keys a CTA holds in shared memory
+  int block_shift;            // log2 of block_size, or -1
 };
 // Returns a cudaError_t.
 int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s);
