@@ -650,12 +650,13 @@ std::tuple<at::Tensor, at::Tensor> gqa_decode_int4(const at::Tensor& q, const at
     p.chunks = here.chunks;
     p.ctas = here.ctas;
     p.direct = here.direct;
-    at::Tensor po, pm;
-    if (!here.direct) {
-      po = at::empty({2 * here.ctas, 8 * here.head_tiles, sh.dim}, q.options().dtype(at::kFloat));
-      pm = at::empty({2 * here.ctas, 8 * here.head_tiles, 2}, q.options().dtype(at::kFloat));
-      p.part_o = po.data_ptr<float>();
-      p.part_ml = pm.data_ptr<float>();
+    at::Tensor ws;
+    if (!here.direct) {  // partial results, their maxima and sums, and the batch's prefix sums
+      const int64_t slots = 2 * here.ctas, rows = 8 * here.head_tiles;
+      ws = at::empty({slots * rows * (sh.dim + 2) + n + 1}, q.options().dtype(at::kFloat));
+      p.part_o = ws.data_ptr<float>();
+      p.part_ml = p.part_o + slots * rows * sh.dim;
+      p.cum = reinterpret_cast<int32_t*>(p.part_ml + slots * rows * 2);
     }
     p.q = static_cast<const char*>(q.data_ptr()) + b0 * q.stride(0) * q.element_size();
     p.out = static_cast<char*>(out.data_ptr()) + b0 * heads * sh.dim * out.element_size();
@@ -712,49 +713,56 @@ std::tuple<at::Tensor, at::Tensor> kv_evict_int4(at::Tensor& kc, at::Tensor& ks,
 }
 
 // ------------------------------------------------------------- int8 linear
-std::tuple<at::Tensor, at::Tensor> int8_quantize(const at::Tensor& x) {
-  const char* op = "int8_quantize";
+void check_int8_rows(const at::Tensor& x, const char* op) {
   check_cuda(x, "x");
   TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), op, ": x [rows, k], dense rows");
-  const int64_t t = x.size(0), k = x.size(1);
+  const int64_t k = x.size(1);
   TORCH_CHECK(k > 0 && k % 16 == 0 && k <= 131072, op, ": k must be a multiple of 16, at most 131072, got ",
               std::to_string(k));
-  TORCH_CHECK(t <= INT32_MAX, op, ": at most 2^31 - 1 rows");
-  const int dt = dtype_code(x);
-  c10::cuda::CUDAGuard g(x.device());
-  auto q = at::empty({t, k}, x.options().dtype(at::kChar));
-  auto scale = at::empty({t}, x.options().dtype(at::kFloat));
-  if (t == 0) return {q, scale};
+  TORCH_CHECK(x.size(0) <= (1 << 24), op, ": at most 2^24 rows");
+  dtype_code(x);
+}
+
+void run_int8_quantize(const at::Tensor& x, int8_t* q, float* scale) {
   const int64_t per16 = 16 / x.element_size();
   const bool vec = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(0) % per16 == 0;
-  C10_CUDA_CHECK((cudaError_t)launch_int8_quantize(q.data_ptr<int8_t>(), scale.data_ptr<float>(), x.data_ptr(),
-                                                   x.stride(0), (int)t, (int)k, vec, dt, stream()));
+  C10_CUDA_CHECK((cudaError_t)launch_int8_quantize(q, scale, x.data_ptr(), x.stride(0), (int)x.size(0),
+                                                   (int)x.size(1), vec, dtype_code(x), stream()));
+}
+
+std::tuple<at::Tensor, at::Tensor> int8_quantize(const at::Tensor& x) {
+  check_int8_rows(x, "int8_quantize");
+  c10::cuda::CUDAGuard g(x.device());
+  auto q = at::empty({x.size(0), x.size(1)}, x.options().dtype(at::kChar));
+  auto scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  if (x.size(0) > 0) run_int8_quantize(x, q.data_ptr<int8_t>(), scale.data_ptr<float>());
   return {q, scale};
 }
 
 at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale,
                        at::ScalarType out_dtype) {
   const char* op = "int8_linear";
-  check_cuda(x, "x");
-  TORCH_CHECK(x.dim() == 2, op, ": x [tokens, k]");
+  check_int8_rows(x, op);
   check_same_device(w, x, op, "w");
   check_same_device(w_scale, x, op, "w_scale");
   TORCH_CHECK(w.scalar_type() == at::kChar && w.dim() == 2 && w.is_contiguous() && w.size(1) == x.size(1) &&
                   reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0, op,
               ": int8 contiguous w [n, k], 16-byte aligned, k as in x");
-  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= (1 << 24) && x.size(0) <= (1 << 24), op, ": 1 <= n <= 2^24, tokens <= 2^24");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= (1 << 24), op, ": 1 <= n <= 2^24");
   TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.dim() == 1 && w_scale.size(0) == w.size(0) &&
                   (w.size(0) <= 1 || w_scale.stride(0) == 1), op, ": fp32 w_scale [n]");
   TORCH_CHECK(out_dtype == at::kBFloat16 || out_dtype == at::kHalf || out_dtype == at::kFloat, op,
               ": bf16, fp16 or fp32 output");
   c10::cuda::CUDAGuard g(x.device());
-  auto [q, s] = int8_quantize(x);
-  auto y = at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
-  if (x.size(0) == 0) return y;
+  const int64_t t = x.size(0), k = x.size(1);
+  auto y = at::empty({t, w.size(0)}, x.options().dtype(out_dtype));
+  if (t == 0) return y;
+  auto ws = at::empty({t * k + t * 4}, x.options().dtype(at::kChar));  // the int8 rows, then their scales
   Int8GemmParams p{};
   p.y = y.data_ptr();
-  p.xq = q.data_ptr<int8_t>();
-  p.xs = s.data_ptr<float>();
+  p.xq = ws.data_ptr<int8_t>();
+  p.xs = reinterpret_cast<const float*>(p.xq + t * k);
+  run_int8_quantize(x, ws.data_ptr<int8_t>(), reinterpret_cast<float*>(ws.data_ptr<int8_t>() + t * k));
   p.w = w.data_ptr<int8_t>();
   p.ws = w_scale.data_ptr<float>();
   p.status = status_ptr_or_null(x);

@@ -658,6 +658,8 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   int64_t at = 0, end = 1;  // direct: one (sequence, head chunk) per CTA
   if (!p.direct) {
     cost_prefix(p, cum, s_warp);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= p.batch; i += kDecThreads) p.cum[i] = cum[i];
     const int64_t total = (int64_t)cum[p.batch] * heads_v;
     const int64_t share = share_of(total, gridDim.x);
     at = min(total, blockIdx.x * share);
@@ -783,40 +785,18 @@ constexpr int kJoinWarps = 8;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Kv4DecodeParams p) {
   constexpr int H = NT * 8, kThreads = kJoinWarps * 32, V = D / 32;  // dims a lane holds
-  __shared__ int s_sum[2][kJoinWarps];
   __shared__ float s_ml[2][kJoinWarps], s_o[kJoinWarps][D];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int heads_v = p.kv_heads * p.chunks, group = p.heads / p.kv_heads;
   const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int hv = head / group * p.chunks + head % group / H, h = head % group % H;
   const int tiles = tiles_of(seq_len_of(p, b));
-  int before = 0, all = 0;
-  for (int i = threadIdx.x; i < p.batch; i += kThreads) {
-    const int t = cost_of(tiles_of(seq_len_of(p, i)));
-    all += t;
-    if (i < b) before += t;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if (lane == 0) {
-    s_sum[0][warp] = before;
-    s_sum[1][warp] = all;
-  }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    before += s_sum[0][w];
-    all += s_sum[1][w];
-  }
+  pdl_wait();
+  const int before = p.cum[b], all = p.cum[p.batch];  // left by the decode's first CTA
   const int64_t share = share_of((int64_t)all * heads_v, p.ctas);
   const int64_t start = (int64_t)before * heads_v + (int64_t)hv * cost_of(tiles) + kPieceCost;
   const int64_t c0 = start / share;
   const int n = tiles > 0 ? (int)((start + tiles - 1) / share - c0) + 1 : 0;
-  pdl_wait();
   if (n == 1) return;  // one CTA had all of it and wrote the result
   float m = kLowest, l = 0.f, o[V] = {};
 #pragma unroll 4

@@ -126,22 +126,11 @@ __global__ void __launch_bounds__(kThreads) write_kernel(Kv4WriteParams p) {
   if (p.scores != nullptr && live && part == 0) p.scores[dst] = 0.f;
 }
 
-template <typename T>
-AFD_DEVICE void store_values(T* dst, uint32_t word, uint32_t pair) {
-  constexpr int N = Vec16<T>::N;
-  const float step = pair_step(pair), zero = pair_zero(pair);
-#pragma unroll
-  for (int u = 0; u < 8 / N; ++u) {
-    Vec16<T> v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(fmaf((float)((word >> (4 * (u * N + i))) & 15u), step, zero));
-    store16(dst + u * N, v);
-  }
-}
-
+// A thread writes one 16-byte vector of K and of V: neighbouring lanes,
+// neighbouring vectors.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) read_kernel(Kv4ReadParams p) {
-  constexpr int kParts = D / 8, kRows = kThreads / kParts;
+  constexpr int N = Vec16<T>::N, kParts = D / N, kRows = kThreads / kParts;
   const uint32_t part = threadIdx.x % kParts;
   const uint32_t row = blockIdx.x * kRows + threadIdx.x / kParts;
   if (row >= (uint32_t)p.tokens * (uint32_t)p.kv_heads) return;
@@ -152,18 +141,26 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Kv4ReadParams p) {
     if (part == 0 && p.status != nullptr) atomicExch(p.status, kStatusBadIndex);
   } else {
     const int64_t src = cache_row(slot, head, p.kv_heads, p.block_size, p.block_shift);
-    kw = reinterpret_cast<const uint32_t*>(p.k_codes)[src * kParts + part];
-    vw = reinterpret_cast<const uint32_t*>(p.v_codes)[src * kParts + part];
-    kp = p.k_scale[src * (D / kGroup) + part / 8];
-    vp = p.v_scale[src * (D / kGroup) + part / 8];
+    const int64_t word = src * (D / 8) + part * N / 8, pair = src * (D / kGroup) + part * N / kGroup;
+    kw = reinterpret_cast<const uint32_t*>(p.k_codes)[word] >> (part * N % 8 * 4);
+    vw = reinterpret_cast<const uint32_t*>(p.v_codes)[word] >> (part * N % 8 * 4);
+    kp = p.k_scale[pair];
+    vp = p.v_scale[pair];
   }
-  const int64_t at = (int64_t)row * D + part * 8;
-  store_values(reinterpret_cast<T*>(p.k) + at, kw, kp);
-  store_values(reinterpret_cast<T*>(p.v) + at, vw, vp);
+  Vec16<T> k, v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    k.v[i] = from_f32<T>(fmaf((float)((kw >> (4 * i)) & 15u), pair_step(kp), pair_zero(kp)));
+    v.v[i] = from_f32<T>(fmaf((float)((vw >> (4 * i)) & 15u), pair_step(vp), pair_zero(vp)));
+  }
+  const int64_t at = (int64_t)row * D + part * N;
+  store16(reinterpret_cast<T*>(p.k) + at, k);
+  store16(reinterpret_cast<T*>(p.v) + at, v);
 }
 
-template <int D> dim3 row_grid(int64_t rows) {
-  constexpr int kRows = kThreads / (D / 8);
+// The grid over rows of D values, N of them a thread.
+template <int D, int N> dim3 row_grid(int64_t rows) {
+  constexpr int kRows = kThreads / (D / N);
   return dim3((unsigned)((rows + kRows - 1) / kRows));
 }
 int shift_of(int block_size) { return (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1; }
@@ -173,9 +170,9 @@ void write(Kv4WriteParams p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.tokens * p.kv_heads;
   p.block_shift = shift_of(p.block_size);
   switch (p.dim) {
-    case 64: write_kernel<T, 64><<<row_grid<64>(rows), kThreads, 0, s>>>(p); break;
-    case 128: write_kernel<T, 128><<<row_grid<128>(rows), kThreads, 0, s>>>(p); break;
-    default: write_kernel<T, 256><<<row_grid<256>(rows), kThreads, 0, s>>>(p);
+    case 64: write_kernel<T, 64><<<row_grid<64, 8>(rows), kThreads, 0, s>>>(p); break;
+    case 128: write_kernel<T, 128><<<row_grid<128, 8>(rows), kThreads, 0, s>>>(p); break;
+    default: write_kernel<T, 256><<<row_grid<256, 8>(rows), kThreads, 0, s>>>(p);
   }
 }
 template <typename T>
@@ -183,9 +180,9 @@ void read(Kv4ReadParams p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.tokens * p.kv_heads;
   p.block_shift = shift_of(p.block_size);
   switch (p.dim) {
-    case 64: read_kernel<T, 64><<<row_grid<64>(rows), kThreads, 0, s>>>(p); break;
-    case 128: read_kernel<T, 128><<<row_grid<128>(rows), kThreads, 0, s>>>(p); break;
-    default: read_kernel<T, 256><<<row_grid<256>(rows), kThreads, 0, s>>>(p);
+    case 64: read_kernel<T, 64><<<row_grid<64, Vec16<T>::N>(rows), kThreads, 0, s>>>(p); break;
+    case 128: read_kernel<T, 128><<<row_grid<128, Vec16<T>::N>(rows), kThreads, 0, s>>>(p); break;
+    default: read_kernel<T, 256><<<row_grid<256, Vec16<T>::N>(rows), kThreads, 0, s>>>(p);
   }
 }
 

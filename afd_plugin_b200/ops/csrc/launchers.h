@@ -403,6 +403,7 @@ struct Kv4DecodeParams {
   int64_t table_stride;
   float* part_o;              // [2 * ctas, 8 * head_tiles, dim] (not direct)
   float* part_ml;             // [2 * ctas, 8 * head_tiles, 2]
+  int32_t* cum;               // [batch + 1] scratch (not direct)
   int* status;                // or null
   int batch, heads, kv_heads, dim, block_size, num_blocks, max_blocks;
   int head_tiles, chunks, ctas, direct;  // from the plan
