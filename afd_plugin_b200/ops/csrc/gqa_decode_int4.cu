@@ -30,6 +30,7 @@
 //
 // Scores: a second pass over K alone, with the joined log-sum-exp, adds each
 // position's probability (summed over the group's query heads) to its score.
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -45,7 +46,7 @@ constexpr int kWarps = 4;
 constexpr int kStages = 3;       // of kTiles tiles each
 constexpr int kScoreStages = 4;  // of one tile's K
 constexpr int kDecThreads = kWarps * 32;
-constexpr int kMaxBatch = 2048;      // sequences per launch (their prefix sums sit in shared memory)
+constexpr int kMaxBatch = 256;       // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
 constexpr float kStepTop = 512.f;    // scaled steps stay below this (times 2^kLazy: fp16 factors below 2^15)
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
@@ -78,6 +79,10 @@ template <int D, int NT> constexpr int kTiles = D * NT <= 128 ? 2 : 1;
 // CTAs one SM holds (their registers bound it).  Measured at 16 sequences of
 // 50 - 131 K positions, D = 128: see the launcher.
 template <int D, int NT> constexpr int kResident = D * NT <= 128 ? 3 : 2;
+// Row lengths of query heads and of results in shared memory, padded so that
+// the lanes of one access fall on different banks.
+template <int D> constexpr int kQueryLd = D + 8;
+template <int D> constexpr int kRedLd = D + 4;
 template <int D> constexpr int kRow4 = D == 256 ? 64 : (D == 128 ? 32 : 0);
 
 // The 8 codes of a word as fp16 pairs c - 8: v[i] = codes i and i + 4.  OR-ing
@@ -248,8 +253,9 @@ struct TileWalk {
   uint32_t block_codes, block_pairs;  // bytes of a block's codes and pairs
   int pg, in, per_block, last_block, blk[U];
 
-  AFD_DEVICE TileWalk(const Kv4DecodeParams& p, int b, int kv_head, int first, int lane)
-      : table(p.block_table + (int64_t)b * p.table_stride), last_block(p.num_blocks - 1) {
+  AFD_DEVICE void start(const Kv4DecodeParams& p, int b, int kv_head, int first, int lane) {
+    table = p.block_table + (int64_t)b * p.table_stride;
+    last_block = p.num_blocks - 1;
     const uint32_t rows = (uint32_t)kv_head * p.block_size;
     kc = p.k_codes + (size_t)rows * (D / 2) + lane * 16;
     vc = p.v_codes + (size_t)rows * (D / 2) + lane * 16;
@@ -343,16 +349,19 @@ struct Query {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const T* row = sq + (t * 8 + g) * D + c * 16;
+      const T* row = sq + (t * 8 + g) * kQueryLd<D> + c * 16;
       float amax = 0.f;
 #pragma unroll
       for (int j = 0; j < G; ++j) {
+        Vec16<T> x[2];
+        x[0] = load16(row + j * kGroup);
+        x[1] = load16(row + j * kGroup + 8);
         float acc = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float x = to_f32(row[j * kGroup + i]);
-          acc += x;
-          amax = fmaxf(amax, fabsf(x));
+          const float v = to_f32(x[i >> 3].v[i & 7]);
+          acc += v;
+          amax = fmaxf(amax, fabsf(v));
         }
         acc += __shfl_xor_sync(0xffffffffu, acc, 1);
         acc += __shfl_xor_sync(0xffffffffu, acc, 2);
@@ -369,10 +378,15 @@ struct Query {
 #pragma unroll
       for (int j = 0; j < G; ++j) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // word k / 2, code pairs 2 (k % 2) and 2 (k % 2) + 1
-          const T* at = row + j * kGroup + (k >> 1) * 8 + (k & 1) * 2;
-          f[t][j * 4 + k][0] = pack_f16(to_f32(at[0]) * up, to_f32(at[4]) * up);
-          f[t][j * 4 + k][1] = pack_f16(to_f32(at[1]) * up, to_f32(at[5]) * up);
+        for (int w = 0; w < 2; ++w) {  // the lane's word w, code pairs 0 .. 3
+          const Vec16<T> x = load16(row + j * kGroup + w * 8);
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = to_f32(x.v[i]) * up;
+          f[t][j * 4 + w * 2][0] = pack_f16(v[0], v[4]);
+          f[t][j * 4 + w * 2][1] = pack_f16(v[1], v[5]);
+          f[t][j * 4 + w * 2 + 1][0] = pack_f16(v[2], v[6]);
+          f[t][j * 4 + w * 2 + 1][1] = pack_f16(v[3], v[7]);
         }
       }
     }
@@ -432,15 +446,15 @@ template <typename T, int D, int NT>
 AFD_DEVICE void stage_query(T* sq, const Kv4DecodeParams& p, int b, int head0, int heads) {
   const T* q = reinterpret_cast<const T*>(p.q) + b * p.q_sb + head0 * p.q_sh;
   for (int i = threadIdx.x; i < NT * 8 * D; i += blockDim.x) {
-    const int h = i / D;
-    sq[i] = h < heads ? q[h * p.q_sh + i % D] : from_f32<T>(0.f);
+    const int h = i / D, d = i % D;
+    sq[h * kQueryLd<D> + d] = h < heads ? q[h * p.q_sh + d] : from_f32<T>(0.f);
   }
 }
 
-// Unnormalised result of a piece in shared memory -> output or partial.
+// Unnormalised result of a piece in shared memory -> output (slot -1) or partial.
 template <typename T, int D, int NT>
-AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int heads, int64_t slot, bool whole,
-                             const float* red, const float* ml, int nact) {
+AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int heads, int64_t slot, const float* red,
+                             const float* ml, int nact) {
   // ml: [kWarps][NT * 8] maxima, then sums; red: [nact][NT * 8][D], already on the common maximum
   constexpr int H = NT * 8;
   for (int i = threadIdx.x; i < heads * (D / 4); i += kDecThreads) {
@@ -451,13 +465,13 @@ AFD_DEVICE void write_result(const Kv4DecodeParams& p, int b, int head0, int hea
     for (int w = 0; w < nact; ++w) {
       const float f = fast_exp2(ml[w * H + h] - m);
       l = fmaf(ml[(kWarps + w) * H + h], f, l);
-      const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)w * H + h) * D + d4);
+      const float4 v = *reinterpret_cast<const float4*>(red + (w * H + h) * kRedLd<D> + d4);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
       o.w = fmaf(v.w, f, o.w);
     }
-    if (whole) {
+    if (slot < 0) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       T* out = reinterpret_cast<T*>(p.out) + ((int64_t)b * p.heads + head0 + h) * D + d4;
       out[0] = from_f32<T>(o.x * inv);
@@ -506,15 +520,27 @@ struct Acc {
 // comes) holds the steps below 2^9, so the factors stay below 2^15.  A step
 // that set the scale gets 2^5 at least: factors keep full precision down to
 // 2^-19 of it, and below that are off by at most 2^-30 of it.
-template <typename T, int D, int NT, bool kTail>
+template <typename T, int D, int NT, bool kLogits, bool kTail>
 AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t stage, const Places<D>& at,
-                           const Unpack& codes, uint32_t shl16, int left, int lane) {
+                           const Unpack& codes, uint32_t shl16, int left, int lane, float* logits, int64_t logits_ld,
+                           int heads) {
   using R = Ring<D>;
   constexpr int G = D / kGroup, U = kTiles<D, NT>;
   float s[U][NT][4];
 #pragma unroll
   for (int u = 0; u < U; ++u) tile_logits<T, D, NT>(s[u], q, stage + u * R::kStageBytes, at, codes, shl16);
   const int r0 = tile_row(lane >> 2);
+  if constexpr (kLogits) {  // `logits`: this step's first position, head 0 of the chunk
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int h = t * 8 + (lane & 3) * 2 + (i & 1), r = u * kTile + r0 + (i >> 1) * 8;
+          if (h < heads && (!kTail || r < left)) logits[h * logits_ld + r] = s[u][t][i];
+        }
+  }
   uint32_t pr[U][2][G];          // (step, zero) of rows r0 and r0 + 8
   float st[U][2][G], k[U][2][G]; // their steps, and scaled
   bool grow = false;
@@ -640,15 +666,35 @@ AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t s
   }
 }
 
+// Shared memory of a decode CTA: the warps' rings; their results of a piece,
+// merged while the next piece's first tiles are on their way; a chunk of query
+// heads; the batch's prefix sums.  At D = 128 with 8 heads it is 75.3 KB: three
+// CTAs fill the SM's 227 KB.
 template <typename T, int D, int NT>
+struct DecodeSmem {
+  static constexpr int kRing = kWarps * kStages * kTiles<D, NT> * Ring<D>::kStageBytes;
+  static constexpr int kRed = kWarps * NT * 8 * kRedLd<D> * 4;
+  static constexpr int kQuery = NT * 8 * kQueryLd<D> * (int)sizeof(T);
+  static int bytes(int batch, bool direct) { return kRing + kRed + kQuery + (direct ? 0 : (batch + 1) * 4); }
+};
+
+// What a piece is to the loop: its tiles, and whose they are.
+struct Work {
+  int b, t0, t1, n;                  // n: positions of the sequence
+  int kv_head, head0, heads, slot;   // slot: where a partial result goes, or -1 if it is the whole
+};
+
+template <typename T, int D, int NT, bool kLogits>
 __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel(Kv4DecodeParams p) {
   using R = Ring<D>;
+  using S = DecodeSmem<T, D, NT>;
   constexpr int G = D / kGroup, H = NT * 8, U = kTiles<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_warp[kWarps];
   __shared__ float s_ml[2 * kWarps * H];
-  T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
-  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
+  float* const red = reinterpret_cast<float*>(smem + S::kRing);
+  T* const sq = reinterpret_cast<T*>(smem + S::kRing + S::kRed);
+  int* cum = reinterpret_cast<int*>(smem + S::kRing + S::kRed + S::kQuery);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int heads_v = p.kv_heads * p.chunks;
@@ -665,76 +711,98 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
     at = min(total, blockIdx.x * share);
     end = min(total, at + share);
   }
-  while (at < end) {
+  // The next piece of this CTA's share, if there is one.
+  auto take = [&](Work& w) {
     Piece pc;
-    if (p.direct) {
-      pc.b = blockIdx.x / heads_v;
-      pc.hv = blockIdx.x % heads_v;
-      pc.t0 = 0;
-      pc.t1 = pc.tiles = tiles_of(seq_len_of(p, pc.b));
-      pc.next = end;
-    } else {
+    while (true) {
+      if (at >= end) return false;
+      if (p.direct) {
+        pc.b = blockIdx.x / heads_v;
+        pc.hv = blockIdx.x % heads_v;
+        pc.t0 = 0;
+        pc.t1 = pc.tiles = tiles_of(seq_len_of(p, pc.b));
+        at = end;
+        break;
+      }
       pc = piece_at(cum, p.batch, heads_v, at, end);
-      if (pc.t0 == pc.t1) {
-        at = pc.next;
-        continue;
-      }
+      at = pc.next;
+      if (pc.t0 < pc.t1) break;
     }
-    at = pc.next;
-    const int n = seq_len_of(p, pc.b);
-    const int kv_head = pc.hv / p.chunks, group = p.heads / p.kv_heads;
-    const int h_in = pc.hv % p.chunks * H;
-    const int heads = min(H, group - h_in);
-    const int head0 = kv_head * group + h_in;
-    constexpr uint32_t kStep = U * R::kStageBytes;
-    const uint32_t base = smem_u32(smem) + warp * kStages * kStep;
+    const int group = p.heads / p.kv_heads, h_in = pc.hv % p.chunks * H;
+    w.b = pc.b;
+    w.t0 = pc.t0;
+    w.t1 = pc.t1;
+    w.n = seq_len_of(p, pc.b);
+    w.kv_head = pc.hv / p.chunks;
+    w.head0 = w.kv_head * group + h_in;
+    w.heads = min(H, group - h_in);
+    // Only a share's first and last pieces can be parts of a (sequence, head):
+    // one that begins with its first tile goes to the CTA's second slot.
+    w.slot = pc.t0 == 0 && pc.t1 == pc.tiles ? -1 : 2 * (int)blockIdx.x + (pc.t0 == 0 ? 1 : 0);
+    return true;
+  };
 
-    // Fill the ring.  Steps of U tiles of a piece are dealt to the warps in turn.
-    int issue = pc.t0 + warp * U;
-    TileWalk<D, U> walk(p, pc.b, kv_head, issue, lane);
-    walk.fetch(pc.t1 - issue);
-    auto copy_next = [&](uint32_t into) {
-      if (issue < pc.t1) {
+  // Each warp fills its own ring.  Steps of U tiles of a piece are dealt to the
+  // warps in turn.
+  constexpr uint32_t kStep = U * R::kStageBytes, kLast = (kStages - 1) * kStep;
+  const uint32_t base = smem_u32(smem) + warp * kStages * kStep;
+  TileWalk<D, U> walk;
+  int issue = 0, issue_end = 0;
+  auto copy_next = [&](uint32_t into) {
+    if (issue < issue_end) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (issue + u < pc.t1) walk.template load<true>(u, into + u * R::kStageBytes, place.cp, lane);
-        issue += U * kWarps;
-        walk.advance();
-        walk.fetch(pc.t1 - issue);
-      }
-      cp_commit();
-    };
+      for (int u = 0; u < U; ++u)
+        if (issue + u < issue_end) walk.template load<true>(u, into + u * R::kStageBytes, place.cp, lane);
+      issue += U * kWarps;
+      walk.advance();
+      walk.fetch(issue_end - issue);
+    }
+    cp_commit();
+  };
+  auto begin = [&](const Work& w) {
+    issue = w.t0 + warp * U;
+    issue_end = w.t1;
+    walk.start(p, w.b, w.kv_head, issue, lane);
+    walk.fetch(issue_end - issue);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) copy_next(base + s * kStep);
-    stage_query<T, D, NT>(sq, p, pc.b, head0, heads);
-    check_blocks(p, pc.b, pc.t0, pc.t1);
-    __syncthreads();
+    check_blocks(p, w.b, w.t0, w.t1);
+  };
+
+  Work w, next;
+  bool more = take(w);
+  if (more) {
+    begin(w);
+    stage_query<T, D, NT>(sq, p, w.b, w.head0, w.heads);
+  }
+  while (more) {
+    __syncthreads();  // this piece's query is staged, the last one's results are written
     Query<T, D, NT> q;
     q.load(sq, p.scale_log2, lane);
-
     Acc<D, NT> acc;
     acc.clear();
-    constexpr uint32_t kLast = (kStages - 1) * kStep;
+    float* logits = nullptr;
+    if constexpr (kLogits) logits = p.logits + (int64_t)(w.b * p.heads + w.head0) * p.logits_ld;
     uint32_t st = base, into = base + kLast;
-    for (int tile = pc.t0 + warp * U; tile < pc.t1; tile += U * kWarps) {
+    for (int tile = w.t0 + warp * U; tile < w.t1; tile += U * kWarps) {
       cp_wait<kStages - 2>();
       __syncwarp();
       copy_next(into);  // into the stage that the previous step has left
       // a piece that ends before its sequence may end inside a step
-      const int left = min(n, pc.t1 * kTile) - tile * kTile;
+      const int left = min(w.n, w.t1 * kTile) - tile * kTile;
+      float* const lg = kLogits ? logits + tile * kTile : nullptr;
       if (left >= U * kTile)
-        take_tiles<T, D, NT, false>(acc, q, st, place, codes, p.shl16, left, lane);
+        take_tiles<T, D, NT, kLogits, false>(acc, q, st, place, codes, p.shl16, left, lane, lg, p.logits_ld, w.heads);
       else
-        take_tiles<T, D, NT, true>(acc, q, st, place, codes, p.shl16, left, lane);
+        take_tiles<T, D, NT, kLogits, true>(acc, q, st, place, codes, p.shl16, left, lane, lg, p.logits_ld, w.heads);
       into = st;
       st = st == base + kLast ? base : st + kStep;
       __syncwarp();  // every lane is done with this stage before it is refilled
     }
-    cp_wait<0>();
-    __syncthreads();  // the ring is free: it takes the warps' results
+    more = take(next);
+    if (more) begin(next);  // on its way while this piece is merged
 
-    const int nact = min(kWarps, (pc.t1 - pc.t0 + U - 1) / U);
-    float* red = reinterpret_cast<float*>(smem);
+    const int nact = min(kWarps, (w.t1 - w.t0 + U - 1) / U);
     if (warp < nact) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -754,7 +822,7 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
             s_ml[warp * H + h] = acc.m[t][e];
             s_ml[(kWarps + warp) * H + h] = ls;
           }
-          float* to = red + ((size_t)warp * H + h) * D + g * 8;
+          float* to = red + (warp * H + h) * kRedLd<D> + g * 8;
 #pragma unroll
           for (int j = 0; j < G; ++j) {
             const auto& o = acc.o[t];
@@ -770,12 +838,11 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
       }
     }
     __syncthreads();
-    // Only a share's first and last pieces can be parts of a (sequence, head):
-    // one that begins with its first tile goes to the CTA's second slot.
-    write_result<T, D, NT>(p, pc.b, head0, heads, 2 * (int64_t)blockIdx.x + (pc.t0 == 0 ? 1 : 0),
-                           pc.t0 == 0 && pc.t1 == pc.tiles, red, s_ml, nact);
-    __syncthreads();
+    if (more) stage_query<T, D, NT>(sq, p, next.b, next.head0, next.heads);
+    write_result<T, D, NT>(p, w.b, w.head0, w.heads, w.slot, red, s_ml, nact);
+    w = next;
   }
+  cp_wait<0>();
 }
 
 // Joins the partials of every (sequence, head) that more than one CTA worked
@@ -838,6 +905,40 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Kv4DecodeParams p
   }
 }
 
+// Scores from the logits that the decode left (log2 domain, [batch, heads,
+// logits_ld]): a thread takes a position of one (sequence, KV head) and sums the
+// probabilities of the group's heads.  Adds, not stores: sequences may share
+// blocks.
+constexpr int kScoreThreads = 128, kScorePositions = 256;  // of a block: many small ones, to have many loads in flight
+__global__ void __launch_bounds__(kScoreThreads) add_scores_kernel(Kv4DecodeParams p) {
+  const int b = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+  const int n = seq_len_of(p, b), group = p.heads / p.kv_heads;
+  const int64_t head = (int64_t)b * p.heads + kv_head * group;
+  pdl_wait();
+  for (int64_t first = (int64_t)blockIdx.y * kScorePositions; first < n; first += (int64_t)gridDim.y * kScorePositions) {
+    const int t0 = (int)first + threadIdx.x, t1 = t0 + kScoreThreads;
+    const float* at = p.logits + head * p.logits_ld;
+    float w0 = 0.f, w1 = 0.f;
+#pragma unroll 8
+    for (int h = 0; h < group; ++h) {
+      const float lse = p.lse[head + h] * 1.4426950408889634f;
+      if (t0 < n) w0 += fast_exp2(at[h * p.logits_ld + t0] - lse);
+      if (t1 < n) w1 += fast_exp2(at[h * p.logits_ld + t1] - lse);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = u ? t1 : t0;
+      if (t < n) {
+        const int pg = t / p.block_size;
+        const uint32_t blk = min((unsigned)p.block_table[(int64_t)b * p.table_stride + pg], (unsigned)p.num_blocks - 1u);
+        atomicAdd(p.scores + ((int64_t)blk * p.kv_heads + kv_head) * p.block_size + (t - pg * p.block_size), u ? w1 : w0);
+      }
+    }
+  }
+}
+
+// The same without stored logits, from K once more: for batches whose logits
+// would not fit the workspace.
 // Adds every position's probability to its score.  The same shares of tiles;
 // nothing to merge, since a position is in one tile.
 template <typename T, int D, int NT>
@@ -847,7 +948,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_warp[kWarps];
   T* sq = reinterpret_cast<T*>(smem + p.ring_bytes);
-  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * D * sizeof(T));
+  int* cum = reinterpret_cast<int*>(smem + p.ring_bytes + H * kQueryLd<D> * sizeof(T));
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int c = lane & 3, r0 = tile_row(lane >> 2);
   const int heads_v = p.kv_heads * p.chunks;
@@ -870,7 +971,8 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
     const int head0 = kv_head * group + h_in;
     const uint32_t base = smem_u32(smem) + warp * kScoreStages * R::kHalf;
     int issue = pc.t0 + warp;
-    TileWalk<D, 1> walk(p, pc.b, kv_head, issue, lane);
+    TileWalk<D, 1> walk;
+    walk.start(p, pc.b, kv_head, issue, lane);
     walk.fetch(pc.t1 - issue);
     auto copy_next = [&](uint32_t into) {
       if (issue < pc.t1) {
@@ -896,7 +998,8 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
         lse[t][e] = h < heads ? p.lse[(int64_t)pc.b * p.heads + head0 + h] * 1.4426950408889634f : INFINITY;
       }
     // a second walk, for the scores' addresses
-    TileWalk<D, 1> to(p, pc.b, kv_head, pc.t0 + warp, lane);
+    TileWalk<D, 1> to;
+    to.start(p, pc.b, kv_head, pc.t0 + warp, lane);
     float* const scores = p.scores + (size_t)kv_head * p.block_size;
     constexpr uint32_t kLast = (kScoreStages - 1) * R::kHalf;
     uint32_t st = base, into = base + kLast;
@@ -934,19 +1037,16 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
   }
 }
 
-template <typename T, int D, int NT>
-cudaError_t launch_decode(Kv4DecodeParams p, cudaStream_t s) {
-  constexpr int H = NT * 8;
-  constexpr int ring = kWarps * kStages * kTiles<D, NT> * Ring<D>::kStageBytes, red = kWarps * H * D * 4;
-  p.ring_bytes = ring > red ? ring : red;
-  const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.direct ? 0 : (p.batch + 1) * 4);
+template <typename T, int D, int NT, bool kLogits>
+cudaError_t launch_decode(const Kv4DecodeParams& p, cudaStream_t s) {
+  using S = DecodeSmem<T, D, NT>;
+  auto* kernel = decode_kernel<T, D, NT, kLogits>;
   static PerDeviceOnce attr;
   cudaError_t e = attr.run([&] {
-    return cudaFuncSetAttribute(decode_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(kMaxBatch, false));
   });
   if (e != cudaSuccess) return e;
-  decode_kernel<T, D, NT><<<p.ctas, kDecThreads, smem, s>>>(p);
+  kernel<<<p.ctas, kDecThreads, S::bytes(p.batch, p.direct), s>>>(p);
   if (!p.direct) {
     e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)(p.batch * p.heads)), dim3(kJoinWarps * 32), 0, s, p);
     if (e != cudaSuccess) return e;
@@ -958,11 +1058,11 @@ template <typename T, int D, int NT>
 cudaError_t launch_score(Kv4DecodeParams p, cudaStream_t s) {
   constexpr int H = NT * 8;
   p.ring_bytes = kWarps * kScoreStages * Ring<D>::kHalf;
-  const int smem = p.ring_bytes + H * D * (int)sizeof(T) + (p.batch + 1) * 4;
+  const int smem = p.ring_bytes + H * kQueryLd<D> * (int)sizeof(T) + (p.batch + 1) * 4;
   static PerDeviceOnce attr;
   cudaError_t e = attr.run([&] {
     return cudaFuncSetAttribute(score_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                p.ring_bytes + H * D * (int)sizeof(T) + (kMaxBatch + 1) * 4);
+                                p.ring_bytes + H * kQueryLd<D> * (int)sizeof(T) + (kMaxBatch + 1) * 4);
   });
   if (e != cudaSuccess) return e;
   return launch_pdl(score_kernel<T, D, NT>, dim3(4 * device_sm_count()), dim3(kDecThreads), (size_t)smem, s, p);
@@ -970,9 +1070,15 @@ cudaError_t launch_score(Kv4DecodeParams p, cudaStream_t s) {
 
 template <typename T, int D, int NT>
 cudaError_t run(const Kv4DecodeParams& p, cudaStream_t s) {
-  const cudaError_t e = launch_decode<T, D, NT>(p, s);
+  const cudaError_t e = p.logits != nullptr ? launch_decode<T, D, NT, true>(p, s) : launch_decode<T, D, NT, false>(p, s);
   if (e != cudaSuccess || p.scores == nullptr) return e;
-  return launch_score<T, D, NT>(p, s);
+  if (p.logits == nullptr) return launch_score<T, D, NT>(p, s);
+  // blocks for every position there may be, up to 64 waves; the rest in turn
+  const int64_t chunks = ((int64_t)p.max_blocks * p.block_size + kScorePositions - 1) / kScorePositions;
+  const int64_t most = 1 + (int64_t)64 * 16 * device_sm_count() / (p.batch * p.kv_heads);
+  return launch_pdl(add_scores_kernel,
+                    dim3((unsigned)(p.batch * p.kv_heads), (unsigned)std::min<int64_t>({chunks, most, 65535})),
+                    dim3(kScoreThreads), 0, s, p);
 }
 
 template <typename T>

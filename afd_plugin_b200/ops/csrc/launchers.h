@@ -404,6 +404,8 @@ struct Kv4DecodeParams {
   float* part_o;              // [2 * ctas, 8 * head_tiles, dim] (not direct)
   float* part_ml;             // [2 * ctas, 8 * head_tiles, 2]
   int32_t* cum;               // [batch + 1] scratch (not direct)
+  float* logits;              // [batch, heads, logits_ld] scratch for the scores, or null: K is read again for them
+  int64_t logits_ld;
   int* status;                // or null
   int batch, heads, kv_heads, dim, block_size, num_blocks, max_blocks;
   int head_tiles, chunks, ctas, direct;  // from the plan

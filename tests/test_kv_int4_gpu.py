@@ -121,6 +121,9 @@ CASES = [
     (8, 1, 128, 64, [20000], None),                           # one sequence over every CTA
     (8, 2, 128, 64, [5, 9], 100),                             # short sequences, wide table
     (4, 2, 64, 64, [1] * 2100, 9),                            # more sequences than one launch takes
+    (64, 4, 128, 64, [700, 0, 1500], 16500),                  # a table too wide for stored logits: scores from K again
+    (6, 2, 64, 16, [900, 33, 1], 260000),
+    (8, 1, 256, 64, [100, 700], 65536),
 ]
 
 
@@ -140,7 +143,7 @@ def test_decode(case, dtype):
     out2 = ops.gqa_decode_int4(q, kv, table, lens_t, scale, scores=scores)
     assert torch.equal(out, out2)
     if len(lens) > 100:
-        lens, keep = lens[:3] + lens[2047:2050], [0, 1, 2, 2047, 2048, 2049]
+        lens, keep = lens[:6], [0, 1, 511, 512, 2047, 2099]
         q, table, out, lse = (t[keep] for t in (q, table, out, lse))
         _check_decode(q, kv, table, lens, scale, out, lse)
         return
