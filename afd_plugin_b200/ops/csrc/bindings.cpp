@@ -650,10 +650,10 @@ std::tuple<at::Tensor, at::Tensor> gqa_decode_int4(const at::Tensor& q, const at
     p.chunks = here.chunks;
     p.ctas = here.ctas;
     p.direct = here.direct;
-    // Workspace: partial results, their maxima and sums and the batch's prefix
-    // sums; with scores, the logits (as long as they take at most 512 MB).
+    // Workspace: partial results, their maxima and sums, and which (sequences,
+    // heads) they are of; with scores, the logits (as long as they take at most 512 MB).
     const int64_t slots = here.direct ? 0 : 2 * here.ctas, rows = 8 * here.head_tiles;
-    const int64_t part = slots * rows * (sh.dim + 2) + (here.direct ? 0 : (n + 4) / 4 * 4);
+    const int64_t part = slots * rows * (sh.dim + 2) + 2 * slots;
     p.logits_ld = (max_len + 3) / 4 * 4;
     const int64_t logits = sc != nullptr && n * heads * p.logits_ld <= (127 << 20) ? n * heads * p.logits_ld : 0;
     at::Tensor ws;
@@ -662,7 +662,7 @@ std::tuple<at::Tensor, at::Tensor> gqa_decode_int4(const at::Tensor& q, const at
       ws = at::empty({part + logits}, q.options().dtype(at::kFloat));
       p.part_o = ws.data_ptr<float>();
       p.part_ml = p.part_o + slots * rows * sh.dim;
-      p.cum = reinterpret_cast<int32_t*>(p.part_ml + slots * rows * 2);
+      p.splits = reinterpret_cast<int32_t*>(p.part_ml + slots * rows * 2);
       if (logits > 0) p.logits = p.part_o + part;
     }
     p.q = static_cast<const char*>(q.data_ptr()) + b0 * q.stride(0) * q.element_size();

@@ -50,8 +50,12 @@ constexpr int kMaxBatch = 256;       // sequences per launch (their prefix sums 
 constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
 constexpr float kStepTop = 512.f;    // scaled steps stay below this (times 2^kLazy: fp16 factors below 2^15)
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
-// What a piece costs beside its tiles (pipeline fill, query, merge), in tiles.
-constexpr int kPieceCost = 4;
+// What a piece costs beside its tiles (pipeline fill, query, merge), in tiles,
+// and the steps of all warps that tiles come in.  Measured at 256 sequences of
+// 1 - 4001 positions, D = 256: 119, 107, 101 and 97 us with 4, 10, 16 and 24;
+// at 16 of 2050 and of 50 - 131 K positions 10 and more are alike.
+constexpr int kPieceCost = 16;
+constexpr int kRound = 8;
 constexpr int kMinShare = 8;         // a CTA's share of tiles is not cut below this
 
 template <int D>
@@ -174,7 +178,7 @@ AFD_DEVICE int tile_row(int i) { return (i & 8) | ((i & 7) >> 1) | ((i & 1) << 2
 
 AFD_DEVICE int tiles_of(int n) { return (n + kTile - 1) / kTile; }
 // Length of a (sequence, head chunk) in the order the shares are cut from.
-AFD_DEVICE int cost_of(int tiles) { return tiles > 0 ? tiles + kPieceCost : 0; }
+AFD_DEVICE int cost_of(int tiles) { return tiles > 0 ? (tiles + kRound - 1) / kRound * kRound + kPieceCost : 0; }
 
 // Inclusive prefix sums of the sequences' costs into cum[1 .. batch]
 // (cum[0] = 0); every thread of the block calls this.
@@ -222,8 +226,8 @@ struct Piece {
 // The piece that starts at position `at` of the batch's order and ends at `end`
 // or at its (sequence, head)'s end.  It may hold no tile (t0 == t1), when only
 // a (sequence, head)'s fixed cost fell into the share.
-AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, int64_t end) {
-  int lo = 0, hi = batch - 1;  // largest b with cum[b] * heads_v <= at
+AFD_DEVICE Piece piece_at(const Kv4DecodeParams& p, const int* cum, int heads_v, int64_t at, int64_t end) {
+  int lo = 0, hi = p.batch - 1;  // largest b with cum[b] * heads_v <= at
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if ((int64_t)cum[mid] * heads_v <= at) lo = mid;
@@ -236,9 +240,9 @@ AFD_DEVICE Piece piece_at(const int* cum, int batch, int heads_v, int64_t at, in
   pc.hv = (int)(rem / cost);
   const int v0 = (int)(rem - (int64_t)pc.hv * cost);
   const int v1 = (int)min((int64_t)cost, v0 + (end - at));
-  pc.tiles = cost - kPieceCost;
-  pc.t0 = max(0, v0 - kPieceCost);
-  pc.t1 = max(0, v1 - kPieceCost);
+  pc.tiles = tiles_of(seq_len_of(p, lo));
+  pc.t0 = min(pc.tiles, max(0, v0 - kPieceCost));
+  pc.t1 = min(pc.tiles, max(0, v1 - kPieceCost));
   pc.next = at + (v1 - v0);
   return pc;
 }
@@ -701,16 +705,23 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
   const Places<D> place(lane);
   const Unpack codes{p.mask_lo, p.mask_hi, p.base_f16};
 
-  int64_t at = 0, end = 1;  // direct: one (sequence, head chunk) per CTA
+  int64_t at = 0, end = 1, share = 1;  // direct: one (sequence, head chunk) per CTA
   if (!p.direct) {
     cost_prefix(p, cum, s_warp);
-    if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i <= p.batch; i += kDecThreads) p.cum[i] = cum[i];
     const int64_t total = (int64_t)cum[p.batch] * heads_v;
-    const int64_t share = share_of(total, gridDim.x);
+    share = share_of(total, gridDim.x);
     at = min(total, blockIdx.x * share);
     end = min(total, at + share);
+    // empty sequences have no piece: their results are written here
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+      if (seq_len_of(p, b) == 0) {
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.heads * D;
+        for (int i = threadIdx.x; i < p.heads * D; i += kDecThreads) out[i] = from_f32<T>(0.f);
+        if (p.lse != nullptr)
+          for (int i = threadIdx.x; i < p.heads; i += kDecThreads) p.lse[(int64_t)b * p.heads + i] = -INFINITY;
+      }
   }
+  int4 split = make_int4(0, 0, 0, 0);  // for the join: sequence, first head, heads, pieces
   // The next piece of this CTA's share, if there is one.
   auto take = [&](Work& w) {
     Piece pc;
@@ -724,7 +735,7 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
         at = end;
         break;
       }
-      pc = piece_at(cum, p.batch, heads_v, at, end);
+      pc = piece_at(p, cum, heads_v, at, end);
       at = pc.next;
       if (pc.t0 < pc.t1) break;
     }
@@ -739,6 +750,8 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
     // Only a share's first and last pieces can be parts of a (sequence, head):
     // one that begins with its first tile goes to the CTA's second slot.
     w.slot = pc.t0 == 0 && pc.t1 == pc.tiles ? -1 : 2 * (int)blockIdx.x + (pc.t0 == 0 ? 1 : 0);
+    if (pc.t0 == 0 && pc.t1 < pc.tiles)  // goes on in the CTAs after this one, to that of its last tile
+      split = make_int4(w.b, w.head0, w.heads, 1 + (int)((pc.tiles - pc.t1 + share - 1) / share));
     return true;
   };
 
@@ -843,66 +856,65 @@ __global__ void __launch_bounds__(kDecThreads, (kResident<D, NT>)) decode_kernel
     w = next;
   }
   cp_wait<0>();
+  if (!p.direct && threadIdx.x == 0) *reinterpret_cast<int4*>(p.splits + 4 * blockIdx.x) = split;
 }
 
-// Joins the partials of every (sequence, head) that more than one CTA worked
-// on, and writes the empty sequences.  One block per (sequence, query head):
-// its warps take the pieces in turn, and merge through shared memory.
-constexpr int kJoinWarps = 8;
+// Joins the partials of the (sequences, head chunks) that more than one CTA
+// worked on: block c those of the one that begins in CTA c's share and goes on
+// in the next, if there is one.  kJoinWarps / H warps take a head's pieces in
+// turn and merge through shared memory.
+constexpr int kJoinWarps = 32;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(Kv4DecodeParams p) {
-  constexpr int H = NT * 8, kThreads = kJoinWarps * 32, V = D / 32;  // dims a lane holds
-  __shared__ float s_ml[2][kJoinWarps], s_o[kJoinWarps][D];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int heads_v = p.kv_heads * p.chunks, group = p.heads / p.kv_heads;
-  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
-  const int hv = head / group * p.chunks + head % group / H, h = head % group % H;
-  const int tiles = tiles_of(seq_len_of(p, b));
+  constexpr int H = NT * 8, W = kJoinWarps / H, V = D / 32;  // warps of a head, dims a lane holds
+  __shared__ float s_ml[kJoinWarps][2], s_o[kJoinWarps][D];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, h = warp / W, part = warp % W;
   pdl_wait();
-  const int before = p.cum[b], all = p.cum[p.batch];  // left by the decode's first CTA
-  const int64_t share = share_of((int64_t)all * heads_v, p.ctas);
-  const int64_t start = (int64_t)before * heads_v + (int64_t)hv * cost_of(tiles) + kPieceCost;
-  const int64_t c0 = start / share;
-  const int n = tiles > 0 ? (int)((start + tiles - 1) / share - c0) + 1 : 0;
-  if (n == 1) return;  // one CTA had all of it and wrote the result
+  const int4 split = *reinterpret_cast<const int4*>(p.splits + 4 * blockIdx.x);  // sequence, first head, heads, pieces
+  if (split.w == 0) return;
   float m = kLowest, l = 0.f, o[V] = {};
-#pragma unroll 4
-  for (int k = warp; k < n; k += kJoinWarps) {
-    // piece k's slot: the first begins with the first tile, the others begin shares
-    const int64_t slot = (2 * (c0 + k) + (k == 0 ? 1 : 0)) * H + h;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-    float v[V];
+  if (h < split.z) {
+#pragma unroll 8
+    for (int k = part; k < split.w; k += W) {
+      // the first piece is in its CTA's second slot, the others begin shares
+      const int64_t slot = (2 * (int64_t)(blockIdx.x + k) + (k == 0 ? 1 : 0)) * H + h;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+      float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = p.part_o[slot * D + i * 32 + lane];
-    const float mx = fmaxf(m, ml.x), f = fast_exp2(m - mx), g = fast_exp2(ml.x - mx);
-    m = mx;
-    l = l * f + ml.y * g;
+      for (int i = 0; i < V; ++i) v[i] = p.part_o[slot * D + i * 32 + lane];
+      const float mx = fmaxf(m, ml.x), f = fast_exp2(m - mx), g = fast_exp2(ml.x - mx);
+      m = mx;
+      l = l * f + ml.y * g;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = o[i] * f + v[i] * g;
+      for (int i = 0; i < V; ++i) o[i] = o[i] * f + v[i] * g;
+    }
   }
   if (lane == 0) {
-    s_ml[0][warp] = m;
-    s_ml[1][warp] = l;
+    s_ml[warp][0] = m;
+    s_ml[warp][1] = l;
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) s_o[warp][i * 32 + lane] = o[i];
   __syncthreads();
-  m = kLowest;
+  if (part != 0 || h >= split.z) return;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, s_ml[0][w]);
-  for (int d = threadIdx.x; d < D; d += kThreads) {
-    l = 0.f;
-    float sum = 0.f;
+  for (int w = 1; w < W; ++w) m = fmaxf(m, s_ml[warp + w][0]);
+  l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float f = fast_exp2(s_ml[0][w] - m);
-      l = fmaf(s_ml[1][w], f, l);
-      sum = fmaf(s_o[w][d], f, sum);
-    }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    reinterpret_cast<T*>(p.out)[((int64_t)b * p.heads + head) * D + d] = from_f32<T>(sum * inv);
-    if (d == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.heads + head] = (m + log2f(l)) * 0.6931471805599453f;
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float f = fast_exp2(s_ml[warp + w][0] - m);
+    l = fmaf(s_ml[warp + w][1], f, l);
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = fmaf(s_o[warp + w][i * 32 + lane], f, o[i]);
   }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int64_t row = (int64_t)split.x * p.heads + split.y + h;
+  T* out = reinterpret_cast<T*>(p.out) + row * D;
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i * 32 + lane] = from_f32<T>(o[i] * inv);
+  if (lane == 0 && p.lse != nullptr) p.lse[row] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // Scores from the logits that the decode left (log2 domain, [batch, heads,
@@ -961,7 +973,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) score_kernel(Kv4DecodeParams p
   const int64_t end = min(total, at + share);
   pdl_wait();  // the log-sum-exps of the decode
   while (at < end) {
-    const Piece pc = piece_at(cum, p.batch, heads_v, at, end);
+    const Piece pc = piece_at(p, cum, heads_v, at, end);
     at = pc.next;
     if (pc.t0 == pc.t1) continue;
     const int n = seq_len_of(p, pc.b);
@@ -1048,7 +1060,7 @@ cudaError_t launch_decode(const Kv4DecodeParams& p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   kernel<<<p.ctas, kDecThreads, S::bytes(p.batch, p.direct), s>>>(p);
   if (!p.direct) {
-    e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)(p.batch * p.heads)), dim3(kJoinWarps * 32), 0, s, p);
+    e = launch_pdl(join_kernel<T, D, NT>, dim3((unsigned)p.ctas), dim3(kJoinWarps * 32), 0, s, p);
     if (e != cudaSuccess) return e;
   }
   return cudaGetLastError();

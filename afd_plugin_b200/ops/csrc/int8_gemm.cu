@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (row < a.t) part[(c0 + j) * kBM + quarter * 32 + lane] = v[j];
+            part[(c0 + j) * kBM + quarter * 32 + lane] = v[j];
         }
       } else {
 #pragma unroll 1
@@ -372,35 +372,46 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     cluster.sync();
     int m, n;
     tile_at(a, first, m, n);
-    // Units of 8 channels of one token; CTA r takes channel octets r, r +
+    // Units of 8 channels of 4 tokens; CTA r takes channel octets r, r +
     // splits, ..., its threads tokens innermost.
-    const int toks = min(kBM, a.t - m * kBM);
+    const int toks = min(kBM, a.t - m * kBM), quads = (toks + 3) / 4;
     const int octets = (BN / 8 - split_rank + splits - 1) / splits;
-    for (int i = threadIdx.x; i < toks * octets; i += kThreads) {
-      const int tok = i % toks, c = (split_rank + i / toks * splits) * 8;
+    for (int i = threadIdx.x; i < quads * octets; i += kThreads) {
+      const int tok = i % quads * 4, c = (split_rank + i / quads * splits) * 8;
       const int n0 = n * BN + c;
       if (n0 >= a.n) continue;
-      int v[8] = {};
+      int v[4][8] = {};
       for (int r = 0; r < splits; ++r) {
-        const int* part = cluster.map_shared_rank(reinterpret_cast<int*>(sm.x[0]), r);
+        const int* part = cluster.map_shared_rank(reinterpret_cast<int*>(sm.x[0]), r) + c * kBM + tok;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += part[(c + j) * kBM + tok];
-      }
-      const float xs = a.xs[m * kBM + tok];
-      T* y = reinterpret_cast<T*>(a.y) + (int64_t)(m * kBM + tok) * a.n + n0;
-      if (a.out_vec && n0 + 8 <= a.n) {
-        constexpr int N = Vec16<T>::N;
-#pragma unroll
-        for (int u = 0; u < 8 / N; ++u) {
-          Vec16<T> o;
-#pragma unroll
-          for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>((float)v[u * N + j] * (xs * sm.ws[0][c + u * N + j]));
-          store16(y + u * N, o);
+        for (int j = 0; j < 8; ++j) {
+          const int4 x = *reinterpret_cast<const int4*>(part + j * kBM);
+          v[0][j] += x.x;
+          v[1][j] += x.y;
+          v[2][j] += x.z;
+          v[3][j] += x.w;
         }
-      } else {
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (n0 + j < a.n) y[j] = from_f32<T>((float)v[j] * (xs * sm.ws[0][c + j]));
+      for (int q = 0; q < 4; ++q) {
+        const int row = m * kBM + tok + q;
+        if (row >= a.t) break;
+        const float xs = a.xs[row];
+        T* y = reinterpret_cast<T*>(a.y) + (int64_t)row * a.n + n0;
+        if (a.out_vec && n0 + 8 <= a.n) {
+          constexpr int N = Vec16<T>::N;
+#pragma unroll
+          for (int u = 0; u < 8 / N; ++u) {
+            Vec16<T> o;
+#pragma unroll
+            for (int j = 0; j < N; ++j) o.v[j] = from_f32<T>((float)v[q][u * N + j] * (xs * sm.ws[0][c + u * N + j]));
+            store16(y + u * N, o);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n0 + j < a.n) y[j] = from_f32<T>((float)v[q][j] * (xs * sm.ws[0][c + j]));
+        }
       }
     }
     cluster.sync();  // no CTA's shared memory goes away while another reads it

@@ -403,7 +403,7 @@ struct Kv4DecodeParams {
   int64_t table_stride;
   float* part_o;              // [2 * ctas, 8 * head_tiles, dim] (not direct)
   float* part_ml;             // [2 * ctas, 8 * head_tiles, 2]
-  int32_t* cum;               // [batch + 1] scratch (not direct)
+  int32_t* splits;            // [ctas, 4] scratch, 16-byte aligned (not direct)
   float* logits;              // [batch, heads, logits_ld] scratch for the scores, or null: K is read again for them
   int64_t logits_ld;
   int* status;                // or null
