@@ -62,6 +62,13 @@ class CacheConfig:
     memory_fraction: float = 0.5
     # Reuse the KV blocks of a shared prompt prefix (full-attention models only).
     enable_prefix_caching: bool = False
+    # "int4": grouped-query attention layers cache K and V in 4 bits (``ops.gqa_decode_int4``).
+    kv_cache_dtype: str = "auto"
+    # Cached positions a sequence is cut to, per KV head, once it holds ``kv_budget_slack`` more
+    # (``ops.kv_evict_int4``; needs the 4-bit cache): the last ``kv_recent`` and the most attended.
+    kv_budget: int | None = None
+    kv_recent: int = 128
+    kv_budget_slack: int = 64
 
 
 @dataclass

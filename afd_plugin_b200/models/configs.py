@@ -87,6 +87,9 @@ class ModelArchConfig:
     eos_token_id: tuple[int, ...] = ()
     # "fp8_block": e4m3 weights with 128x128 scales for experts and dense MLPs.
     quant: str | None = None
+    # "int8": the q / k / v and output projections of grouped-query attention as int8 weights with a
+    # scale per output channel, tokens quantised on the fly (quantised at load from any checkpoint).
+    attn_quant: str | None = None
     weight_block_size: tuple[int, int] = (128, 128)
     extra: dict = field(default_factory=dict)
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch import nn
@@ -307,6 +308,42 @@ class MLAAttention(nn.Module):
         return self.tp.all_reduce(ops.linear(o, self.o_proj))
 
 
+class Int4Layer(NamedTuple):
+    """One layer's 4-bit KV cache, with the accumulated attention weight of every cached position
+    when the cache is bounded (:class:`~afd_plugin_b200.runtime.kv_cache.KVCache`)."""
+
+    kv: ops.Int4KV
+    scores: torch.Tensor | None
+
+
+def _project(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor | None) -> torch.Tensor:
+    return ops.linear(x, w) if scale is None else ops.int8_linear(x, w, scale)
+
+
+def _attend_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: AttentionMetadata, cache: Int4Layer,
+                 scale: float) -> torch.Tensor:
+    """Store the step's K / V rows in the 4-bit cache, then attend over it.
+
+    A prefill reads its sequence's stored values back, so every position sees the keys and values
+    that later decode steps see.  With scores, the new positions start at zero and every query of
+    the step, a prompt's included, adds its attention weights.
+    """
+    ops.gqa_cache_write_int4(cache.kv, k, v, meta.slot_mapping, cache.scores)
+    if meta.is_decode:
+        return ops.gqa_decode_int4(q, cache.kv, meta.block_table, meta.seq_lens, scale, scores=cache.scores)
+    o = torch.empty_like(q)
+    bs = cache.kv.block_size
+    for start, end, seq in meta.prefill_seqs or []:
+        pos = torch.arange(int(meta.positions[start:end].max()) + 1, device=q.device)
+        slots = meta.block_table[seq].long()[pos // bs] * bs + pos % bs
+        ks, vs = ops.gqa_cache_read_int4(cache.kv, slots, dtype=q.dtype)
+        o[start:end], weights = ref.gqa_attend(q[start:end], ks, vs, meta.positions[start:end], scale)
+        if cache.scores is not None:
+            heads = torch.arange(weights.shape[0], device=q.device)[:, None]
+            cache.scores.index_put_((slots // bs, heads, slots % bs), weights, accumulate=True)
+    return o
+
+
 class GQAAttention(nn.Module):
     """Grouped-query attention, with per-head QK RMSNorm when ``arch.qk_norm`` (Qwen3);
     without it, the multi-head attention of DeepSeek V1 (``kv heads == heads``)."""
@@ -320,16 +357,28 @@ class GQAAttention(nn.Module):
         self.d = arch.head_dim
         self.scale = arch.softmax_scale
         H = arch.hidden_size
-        self.qkv_proj = _param(((self.nq + 2 * self.nkv) * self.d, H), dtype, device)
+        # int8 projections: integer weights and a scale per output channel (``arch.attn_quant``)
+        if arch.attn_quant not in (None, "int8"):
+            raise ValueError(f"unknown attention projection quantisation {arch.attn_quant!r}")
+        wdtype = torch.int8 if arch.attn_quant == "int8" else dtype
+        self.qkv_proj = _param(((self.nq + 2 * self.nkv) * self.d, H), wdtype, device)
         self.qk_norm = arch.qk_norm
         if self.qk_norm:
             self.q_norm = RMSNorm(self.d, arch.rms_norm_eps, dtype, device)
             self.k_norm = RMSNorm(self.d, arch.rms_norm_eps, dtype, device)
-        self.o_proj = _param((H, self.nq * self.d), dtype, device)
+        self.o_proj = _param((H, self.nq * self.d), wdtype, device)
+        self.qkv_scale = self.o_scale = None
+        if wdtype == torch.int8:
+            self.qkv_scale = _param((self.qkv_proj.shape[0],), torch.float32, device)
+            self.o_scale = _param((H,), torch.float32, device)
 
-    def forward(self, h: torch.Tensor, meta: AttentionMetadata, kv_cache: tuple[torch.Tensor, torch.Tensor], cos_sin):
+    def forward(self, h: torch.Tensor, meta: AttentionMetadata, kv_cache, cos_sin):
         T = h.shape[0]
-        qkv = ops.linear(h, self.qkv_proj)
+        qkv = _project(h, self.qkv_proj, self.qkv_scale)
+        if isinstance(kv_cache, Int4Layer):
+            q, k, v = self._heads(qkv, meta, cos_sin)
+            o = _attend_int4(q, k, v, meta, kv_cache, self.scale)
+            return self.tp.all_reduce(_project(o.reshape(T, self.nq * self.d), self.o_proj, self.o_scale))
         k_cache, v_cache = kv_cache
         if h.is_cuda and cos_sin.shape[-1] == self.d and self.d in (32, 64, 128, 256):
             # QK-norm, RoPE and the cache write of k / v in one kernel
@@ -339,6 +388,13 @@ class GQAAttention(nn.Module):
                                  self.q_norm.eps if self.qk_norm else 1e-6,
                                  meta.positions, cos_sin, k_cache, v_cache, meta.slot_mapping)
             return self._attend(q, meta, k_cache, v_cache, T)
+        q, k, v = self._heads(qkv, meta, cos_sin)
+        ops.gqa_cache_write(k_cache, v_cache, k, v, meta.slot_mapping)
+        return self._attend(q, meta, k_cache, v_cache, T)
+
+    def _heads(self, qkv, meta, cos_sin):
+        """Query, key and value heads of the projection's rows, normalised and rotated."""
+        T = qkv.shape[0]
         q, k, v = qkv.split([self.nq * self.d, self.nkv * self.d, self.nkv * self.d], dim=-1)
         if self.qk_norm:
             q = self.q_norm(q.reshape(T * self.nq, self.d)).view(T, self.nq, self.d)
@@ -349,8 +405,7 @@ class GQAAttention(nn.Module):
         v = v.reshape(T, self.nkv, self.d)
         ops.rope_(q, meta.positions, cos_sin, interleaved=False)
         ops.rope_(k, meta.positions, cos_sin, interleaved=False)
-        ops.gqa_cache_write(k_cache, v_cache, k, v, meta.slot_mapping)
-        return self._attend(q, meta, k_cache, v_cache, T)
+        return q, k, v
 
     def _attend(self, q, meta, k_cache, v_cache, T):
         if meta.is_decode:
@@ -363,8 +418,7 @@ class GQAAttention(nn.Module):
                 o[start:end] = ref.gqa_prefill(
                     q[start:end], k_cache, v_cache, meta.block_table[seq], meta.positions[start:end], self.scale
                 )
-        return self.tp.all_reduce(ops.linear(o.reshape(T, self.nq * self.d), self.o_proj))
-
+        return self.tp.all_reduce(_project(o.reshape(T, self.nq * self.d), self.o_proj, self.o_scale))
 
 
 class GatedDeltaNet(nn.Module):
@@ -492,7 +546,7 @@ class GatedGQAAttention(nn.Module):
         self.qkv_proj.data[:nqd].copy_(g[:, 0].reshape(nqd, -1).to(self.qkv_proj.device, self.qkv_proj.dtype))
         self.qkv_proj.data[nqd : 2 * nqd].copy_(g[:, 1].reshape(nqd, -1).to(self.qkv_proj.device, self.qkv_proj.dtype))
 
-    def forward(self, h: torch.Tensor, meta: AttentionMetadata, kv_cache: tuple[torch.Tensor, torch.Tensor], cos_sin):
+    def forward(self, h: torch.Tensor, meta: AttentionMetadata, kv_cache, cos_sin):
         T = h.shape[0]
         nq, nkv, d = self.nq, self.nkv, self.d
         qkv = ops.linear(h, self.qkv_proj)
@@ -502,6 +556,10 @@ class GatedGQAAttention(nn.Module):
         v = v.reshape(T, nkv, d)
         ops.rope_(q[..., : self.rot], meta.positions, cos_sin, interleaved=False)
         ops.rope_(k[..., : self.rot], meta.positions, cos_sin, interleaved=False)
+        if isinstance(kv_cache, Int4Layer):
+            o = _attend_int4(q, k, v, meta, kv_cache, self.scale)
+            o = o.reshape(T, nq * d) * torch.sigmoid(gate.float()).to(o.dtype)
+            return ops.linear(o, self.o_proj)
         k_cache, v_cache = kv_cache
         ops.gqa_cache_write(k_cache, v_cache, k, v, meta.slot_mapping)
         if meta.is_decode:
@@ -732,6 +790,7 @@ class MoEBlock(nn.Module):
 
 __all__ = [
     "AttentionMetadata",
+    "Int4Layer",
     "DenseMLP",
     "GQAAttention",
     "MLAAttention",

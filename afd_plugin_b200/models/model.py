@@ -125,6 +125,8 @@ class DecoderLayer(nn.Module):
         self.is_moe = arch.is_moe_layer(idx)
         eps = arch.rms_norm_eps
         has_attn = role in ("colocated", "attention")
+        if arch.attn_quant is not None and (arch.is_mla or arch.attn_output_gate or arch.layer_types is not None):
+            raise ValueError("int8 attention projections cover grouped-query attention layers only")
         self.input_layernorm = RMSNorm(arch.hidden_size, eps, dtype, device) if has_attn else None
         self.post_attention_layernorm = RMSNorm(arch.hidden_size, eps, dtype, device) if has_attn else None
         self.self_attn = None
@@ -450,18 +452,47 @@ def _mlp_specs(p: str, mlp: DenseMLP, inter: int) -> Iterator[ParamSpec]:
     yield from _swiglu_specs(p, mlp.w13, mlp.w2, mlp.w13_scale, mlp.w2_scale, inter, hidden)
 
 
+def _int8_rows_of(dst: torch.Tensor, scale: torch.Tensor, dst0: int, src0: int, n: int):
+    """Rows [src0, src0 + n) of a full checkpoint tensor, quantised to int8, into rows [dst0, dst0 + n)."""
+
+    def setter(src: torch.Tensor) -> None:
+        q, s = ref.int8_quantize(src[src0 : src0 + n].float())
+        dst.data[dst0 : dst0 + n].copy_(q.to(dst.device))
+        scale.data[dst0 : dst0 + n].copy_(s.to(scale.device))
+
+    return setter
+
+
+def _int8_cols_of(dst: torch.Tensor, scale: torch.Tensor, src0: int):
+    """Columns [src0, src0 + dst.shape[1]) of a full checkpoint tensor, quantised to int8."""
+
+    def setter(src: torch.Tensor) -> None:
+        q, s = ref.int8_quantize(src[:, src0 : src0 + dst.shape[1]].float())
+        dst.data.copy_(q.to(dst.device))
+        scale.data.copy_(s.to(scale.device))
+
+    return setter
+
+
 def _gqa_specs(p: str, attn: GQAAttention, a: ModelArchConfig) -> Iterator[ParamSpec]:
     """Full checkpoint shapes of ``q/k/v/o_proj`` (+ QK norms); a tensor-parallel rank keeps its heads."""
     d, nq, nkv = attn.d, attn.nq, attn.nkv
     H, nq_all, nkv_all = a.hidden_size, a.num_attention_heads, a.num_key_value_heads
-    yield ParamSpec(p + "q_proj.weight", (nq_all * d, H), _rows_of(attn.qkv_proj, 0, attn.q0 * d, nq * d))
-    yield ParamSpec(p + "k_proj.weight", (nkv_all * d, H), _rows_of(attn.qkv_proj, nq * d, attn.kv0 * d, nkv * d))
-    yield ParamSpec(p + "v_proj.weight", (nkv_all * d, H),
-                    _rows_of(attn.qkv_proj, (nq + nkv) * d, attn.kv0 * d, nkv * d))
+
+    def rows(dst0: int, src0: int, n: int):
+        if attn.qkv_scale is not None:
+            return _int8_rows_of(attn.qkv_proj, attn.qkv_scale, dst0, src0, n)
+        return _rows_of(attn.qkv_proj, dst0, src0, n)
+
+    yield ParamSpec(p + "q_proj.weight", (nq_all * d, H), rows(0, attn.q0 * d, nq * d))
+    yield ParamSpec(p + "k_proj.weight", (nkv_all * d, H), rows(nq * d, attn.kv0 * d, nkv * d))
+    yield ParamSpec(p + "v_proj.weight", (nkv_all * d, H), rows((nq + nkv) * d, attn.kv0 * d, nkv * d))
     if attn.qk_norm:
         yield ParamSpec(p + "q_norm.weight", (d,), _copy(attn.q_norm.weight), "ones")
         yield ParamSpec(p + "k_norm.weight", (d,), _copy(attn.k_norm.weight), "ones")
-    yield ParamSpec(p + "o_proj.weight", (H, nq_all * d), _cols_of(attn.o_proj, attn.q0 * d))
+    yield ParamSpec(p + "o_proj.weight", (H, nq_all * d),
+                    _cols_of(attn.o_proj, attn.q0 * d) if attn.o_scale is None
+                    else _int8_cols_of(attn.o_proj, attn.o_scale, attn.q0 * d))
 
 
 def _gate_specs(p: str, gate) -> Iterator[ParamSpec]:

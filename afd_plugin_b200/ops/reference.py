@@ -518,18 +518,24 @@ def gqa_prefill(
     positions: torch.Tensor,
     scale: float,
 ) -> torch.Tensor:
-    T, Hq, D = q.shape
     n = int(positions.max()) + 1
-    k = gather_paged(k_cache, block_table, n).float()
-    v = gather_paged(v_cache, block_table, n).float()
-    Hkv = k.shape[1]
-    g = Hq // Hkv
-    qf = q.float().view(T, Hkv, g, D)
-    s = torch.einsum("tkgd,nkd->tkgn", qf, k) * scale
+    return gqa_attend(q, gather_paged(k_cache, block_table, n), gather_paged(v_cache, block_table, n), positions,
+                      scale)[0]
+
+
+def gqa_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+               scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention of queries at ``positions`` over the rows ``k`` / ``v [n, kv_heads, d]`` of
+    positions ``0 .. n - 1``: the output, and each row's attention weight summed over the queries
+    and the query heads that share its KV head (``[kv_heads, n]`` fp32)."""
+    T, Hq, D = q.shape
+    n, Hkv = k.shape[:2]
+    qf = q.float().view(T, Hkv, Hq // Hkv, D)
+    s = torch.einsum("tkgd,nkd->tkgn", qf, k.float()) * scale
     mask = torch.arange(n, device=q.device)[None, :] > positions.long()[:, None]
     s = s.masked_fill(mask[:, None, None, :], float("-inf"))
     p = torch.softmax(s, dim=-1)
-    return torch.einsum("tkgn,nkd->tkgd", p, v).reshape(T, Hq, D).to(q.dtype)
+    return torch.einsum("tkgn,nkd->tkgd", p, v.float()).reshape(T, Hq, D).to(q.dtype), p.sum((0, 2))
 
 
 # ------------------------------------------------------ gated delta net (linear attention)

@@ -45,6 +45,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.distributed as dist
 
+from afd_plugin_b200 import ops
 from afd_plugin_b200.engine_config import EngineConfig
 from afd_plugin_b200.runtime.cuda_graph import graph_settings, pad_to_capture_size
 from afd_plugin_b200.runtime.ffn_executor import FFNExecutor, LocalFFNExecutor
@@ -76,6 +77,7 @@ class Request:
     top_logprobs: list = field(default_factory=list)
 
     preemptions: int = 0  # times its blocks were taken back under cache pressure
+    evicted: int = 0  # cached positions given up under a cache budget
 
     @property
     def num_tokens(self) -> int:
@@ -172,9 +174,20 @@ class LLMEngine:
         self.max_blocks_per_seq = math.ceil(mc.max_model_len / self.block_size)
         if num_blocks is None:
             num_blocks = cc.num_blocks or self._auto_num_blocks(model, cc)
+        self.kv_budget = cc.kv_budget
+        if cc.kv_budget is not None:
+            if cc.kv_cache_dtype != "int4":
+                raise ValueError("a KV cache budget needs kv_cache_dtype='int4'")
+            if cc.kv_budget < 1 or not 0 <= cc.kv_recent <= cc.kv_budget or cc.kv_budget_slack < 1:
+                raise ValueError("a KV cache budget needs 0 <= kv_recent <= kv_budget and kv_budget_slack >= 1")
+            if cc.enable_prefix_caching:
+                raise ValueError("a KV cache budget rewrites a sequence's blocks: prefix caching cannot share them")
+            if getattr(engine_config, "async_scheduling", False):
+                raise ValueError("a KV cache budget needs synchronous scheduling")
         # One linear-attention state row per running request plus a padding row.
         self.kv = KVCache(getattr(model, "cache_arch", model.arch), num_blocks, self.block_size, model.dtype,
-                          self.device, max_seqs=self.max_batch + 1)
+                          self.device, max_seqs=self.max_batch + 1, cache_dtype=cc.kv_cache_dtype,
+                          with_scores=cc.kv_budget is not None)
         self._free_state_slots = list(range(self.max_batch - 1, -1, -1))
         self.ffn = ffn_executor or LocalFFNExecutor(model)
         num_ub = engine_config.parallel_config.num_ubatches if engine_config.parallel_config.use_ubatching else 1
@@ -198,6 +211,7 @@ class LLMEngine:
         # called before every step (workers install the peer-heartbeat check)
         self.health_check = None
         self.num_preemptions = 0
+        self.num_evictions = 0  # times a sequence was cut to the cache budget
         # chunked prefill: admitted requests part-way through their prompt
         self.prefilling: list[Request] = []
         self.max_batched_tokens = engine_config.max_num_batched_tokens
@@ -245,6 +259,7 @@ class LLMEngine:
         # HBM bytes a decode step of this rank must move: its weights once, plus the KV
         # rows of the running sequences (added per step from the staged lengths).
         self._weight_bytes = weight_bytes_per_step(model)
+        self._kv_elem_bytes = KVCache.bytes_per_element(model.dtype, cc.kv_cache_dtype)
         self.last_hbm_bytes = 0
         self._last_phase = "decode"
         # noise for sampled requests without their own seed (same seed on every
@@ -260,7 +275,9 @@ class LLMEngine:
         if self.device.type != "cuda":
             return worst
         arch = getattr(model, "cache_arch", model.arch)
-        per_block = max(1, KVCache.bytes_per_block(arch, self.block_size, model.dtype))
+        per_block = max(1, KVCache.bytes_per_block(arch, self.block_size, model.dtype,
+                                                   cache_dtype=cc.kv_cache_dtype,
+                                                   with_scores=cc.kv_budget is not None))
         free, _ = torch.cuda.mem_get_info(self.device)
         state = KVCache.state_bytes_per_seq(arch, model.dtype) * (self.max_batch + 1)
         fit = int((cc.memory_fraction * free - state) // per_block)
@@ -291,6 +308,8 @@ class LLMEngine:
             raise ValueError("prompt + max_tokens exceeds max_model_len")
         if math.ceil((len(prompt) + max_tokens) / self.block_size) > self.kv.allocator.num_blocks - 1:
             raise ValueError("prompt + max_tokens needs more KV blocks than the cache holds")
+        if hold_kv:
+            self._check_transferable()
         req = Request(next(self._ids), list(prompt), max_tokens, hold_kv=hold_kv)
         self._set_sampling(req, sampling)
         self.waiting.append(req)
@@ -379,6 +398,10 @@ class LLMEngine:
                 return r
         return None
 
+    def _check_transferable(self) -> None:
+        if self.kv.int4 is not None:
+            raise ValueError("the 4-bit KV cache is not handed between engines")
+
     # -------------------------------------------- prefill -> decode hand-off
     def export_kv(self, req_id: int) -> bytes:
         """Serialise a held request's cache rows and recurrent state, then free them."""
@@ -420,6 +443,7 @@ class LLMEngine:
         """
         from afd_plugin_b200.runtime import kv_transfer as kt
 
+        self._check_transferable()
         state = kt.unpack(blob)
         if prompt is not None and state.tokens[: state.prompt_len] != list(prompt):
             raise ValueError("the KV payload was prefilled for a different prompt")
@@ -572,6 +596,7 @@ class LLMEngine:
             self._admit_prefilled()
             if not (self.waiting or self.running or self.prefilling) and self.coordinator.size == 1:
                 return {}  # every imported request finished on its transferred token
+        self._keep_budget()
         self._reserve_decode_blocks()
         plan = self._plan_prefill()
         is_prefill = bool(plan)
@@ -672,6 +697,35 @@ class LLMEngine:
             (self._finish(r) if r.finished else self.running.append(r))
         return out
 
+    def _keep_budget(self) -> None:
+        """Cut every running sequence that is ``kv_budget_slack`` positions over the cache budget back
+        to it, in every layer, and give its last blocks back."""
+        if self.kv_budget is None:
+            return
+        cc = self.config.cache_config
+        # the positions cached so far: every token but the last one, less those given up
+        over = [r for r in self.running
+                if r.num_tokens - 1 - r.evicted >= self.kv_budget + cc.kv_budget_slack]
+        if not over:
+            return
+        lens = [r.num_tokens - 1 - r.evicted for r in over]
+        width = max(len(r.blocks) for r in over)
+        table = torch.full((len(over), width), PAD_BLOCK, dtype=torch.int32)
+        for i, r in enumerate(over):
+            table[i, : len(r.blocks)] = torch.tensor(r.blocks, dtype=torch.int32)
+        table = table.to(self.device)
+        lens_t = torch.tensor(lens, dtype=torch.int32, device=self.device)
+        for kv, scores in zip(self.kv.int4, self.kv.scores):
+            ops.kv_evict_int4(kv, scores, table, lens_t, self.kv_budget, cc.kv_recent)
+        keep = math.ceil(self.kv_budget / self.block_size)
+        for r, n in zip(over, lens):
+            r.evicted += n - self.kv_budget
+            self.kv.allocator.free(r.blocks[keep:])
+            del r.blocks[keep:]
+        # a sequence may come back to a block count it had, with other blocks
+        self._row_key = [None] * self.max_batch
+        self.num_evictions += len(over)
+
     def _blocks_short(self, r: Request) -> int:
         """Blocks ``r`` still lacks to prefill its KV tokens and decode one position."""
         return max(0, math.ceil((len(r.kv_tokens) + 1) / self.block_size) - len(r.blocks))
@@ -680,6 +734,7 @@ class LLMEngine:
         """Take back a running request's blocks; it is recomputed from its tokens when re-admitted."""
         self._release(r)
         r.cached_len = 0
+        r.evicted = 0
         r.preemptions += 1
         self.num_preemptions += 1
         self.waiting.insert(0, r)
@@ -691,7 +746,7 @@ class LLMEngine:
         i = 0
         while i < len(self.running):
             r = self.running[i]
-            need = (r.num_tokens - 1) // bs + 1 - len(r.blocks)
+            need = (r.num_tokens - 1 - r.evicted) // bs + 1 - len(r.blocks)
             if need <= 0:
                 i += 1
                 continue
@@ -735,14 +790,15 @@ class LLMEngine:
         bs = self.block_size
         B = len(reqs)
         pos = [r.num_tokens - 1 + lag for r in reqs]
-        for r, p in zip(reqs, pos):
+        place = [p - r.evicted for r, p in zip(reqs, pos)]  # in the cache
+        for r, p in zip(reqs, place):
             if len(r.blocks) * bs <= p:
                 self._ensure_blocks(r, p + 1)
         if not lag:
             self._n_ids[:B] = [r.output[-1] if r.output else r.prompt[-1] for r in reqs]
         self._n_pos[:B] = pos
-        self._n_slot[:B] = [r.blocks[p // bs] * bs + p % bs for r, p in zip(reqs, pos)]
-        self._n_lens[:B] = self._n_pos[:B] + 1
+        self._n_slot[:B] = [r.blocks[p // bs] * bs + p % bs for r, p in zip(reqs, place)]
+        self._n_lens[:B] = [p + 1 for p in place]
         self._n_state[:B] = [r.state_slot for r in reqs]
         table, keys = self._n_table, self._row_key
         for i, r in enumerate(reqs):
@@ -791,7 +847,7 @@ class LLMEngine:
         from afd_plugin_b200.utils.roofline import kv_bytes_per_step
 
         self.last_hbm_bytes = self._weight_bytes + kv_bytes_per_step(getattr(self.model, "cache_arch", self.model.arch), int(self._h_lens[:B].sum()),
-                                                                      elem_bytes=self.model.dtype.itemsize)
+                                                                      elem_bytes=self._kv_elem_bytes)
         flags = {}
         if len(votes) > 1:
             sp = ubatch_splits(run_b, self.runner.num_ubatches)
@@ -913,7 +969,7 @@ class LLMEngine:
 
         self.last_hbm_bytes = self._weight_bytes + kv_bytes_per_step(getattr(self.model, "cache_arch", self.model.arch),
                                                                       int(self._h_lens[:B].sum()),
-                                                                      elem_bytes=self.model.dtype.itemsize)
+                                                                      elem_bytes=self._kv_elem_bytes)
         nxt = self.runner.decode_step(run_b, use_graph=use_graph, **flags)
         if any(not r.sampling.greedy for r in launch):
             # drawn on the device from this step's logits, before the next replay overwrites them

@@ -4,7 +4,9 @@ MLA layers cache one ``kv_lora + rope`` latent row per token
 (``[L, blocks, block_size, 576]`` for DeepSeek), plus the sparse-attention
 indexer's key row when the model has one (``index_k``, DeepSeek-V3.2 /
 GLM-MoE-DSA); GQA layers cache K and V
-(``[L, blocks, block_size, kv_heads, head_dim]`` each).  A token's slot is
+(``[L, blocks, block_size, kv_heads, head_dim]`` each), or in 4 bits
+(``cache_dtype="int4"``: ``int4``, one :class:`~afd_plugin_b200.ops.Int4KV`
+per layer, and ``scores`` when the cache is bounded).  A token's slot is
 ``block_id * block_size + offset``.
 """
 
@@ -15,6 +17,10 @@ from collections import OrderedDict
 import torch
 
 from afd_plugin_b200.models.configs import ModelArchConfig
+from afd_plugin_b200.models.layers import Int4Layer
+from afd_plugin_b200.ops import Int4KV
+from afd_plugin_b200.ops.kv_int4 import INT4_HEAD_DIMS, int4_kv_cache
+from afd_plugin_b200.ops.reference import INT4_GROUP
 
 
 class BlockAllocator:
@@ -139,7 +145,13 @@ class KVCache:
         device: torch.device | str,
         *,
         max_seqs: int = 1,
+        cache_dtype: str = "auto",
+        with_scores: bool = False,
     ):
+        if cache_dtype not in ("auto", "int4"):
+            raise ValueError(f"unknown KV cache type {cache_dtype!r} (auto or int4)")
+        if with_scores and cache_dtype != "int4":
+            raise ValueError("position scores belong to the 4-bit KV cache")
         self.arch = arch
         self.num_blocks = num_blocks
         self.block_size = block_size
@@ -148,7 +160,17 @@ class KVCache:
         self._kv_index = {layer: i for i, layer in enumerate(attn_layers)}
         L = len(attn_layers)
         self.index_k = None
-        if arch.is_mla:
+        self.int4: list[Int4KV] | None = None
+        self.scores = None
+        if cache_dtype == "int4":
+            if arch.is_mla or arch.head_dim not in INT4_HEAD_DIMS:
+                raise ValueError(f"the 4-bit KV cache covers grouped-query attention with head dims {INT4_HEAD_DIMS}")
+            self.k = self.v = self.kv = None
+            self.int4 = [int4_kv_cache(num_blocks, block_size, arch.num_key_value_heads, arch.head_dim, device)
+                         for _ in range(L)]
+            if with_scores:
+                self.scores = torch.zeros(L, num_blocks, arch.num_key_value_heads, block_size, device=device)
+        elif arch.is_mla:
             self.kv = torch.zeros(L, num_blocks, block_size, arch.kv_lora_rank + arch.qk_rope_head_dim,
                                   dtype=dtype, device=device)
             self.k = self.v = None
@@ -176,6 +198,8 @@ class KVCache:
             j = self._state_index[i]
             return (self.conv_state[j], self.ssm_state[j])
         j = self._kv_index[i]
+        if self.int4 is not None:
+            return Int4Layer(self.int4[j], None if self.scores is None else self.scores[j])
         if self.index_k is not None:
             return (self.kv[j], self.index_k[j])
         if self.kv is not None:
@@ -183,9 +207,18 @@ class KVCache:
         return (self.k[j], self.v[j])
 
     @staticmethod
-    def bytes_per_block(arch: ModelArchConfig, block_size: int, dtype: torch.dtype) -> int:
-        elem = torch.empty((), dtype=dtype).element_size()
-        return len(arch.full_attention_layers) * block_size * arch.kv_cache_width * elem
+    def bytes_per_block(arch: ModelArchConfig, block_size: int, dtype: torch.dtype, *, cache_dtype: str = "auto",
+                        with_scores: bool = False) -> int:
+        elem = KVCache.bytes_per_element(dtype, cache_dtype)
+        row = arch.kv_cache_width * elem + (4 * arch.num_key_value_heads if with_scores else 0)
+        return int(len(arch.full_attention_layers) * block_size * row)
+
+    @staticmethod
+    def bytes_per_element(dtype: torch.dtype, cache_dtype: str = "auto") -> float:
+        """Cache bytes one K / V value takes: 4-bit codes share 4 bytes of step and zero per group."""
+        if cache_dtype == "int4":
+            return 0.5 + 4 / INT4_GROUP
+        return torch.empty((), dtype=dtype).element_size()
 
     @staticmethod
     def state_bytes_per_seq(arch: ModelArchConfig, dtype: torch.dtype) -> int:
@@ -200,12 +233,18 @@ class KVCache:
 
     def fill_random_(self, seed: int = 0, std: float = 1.0) -> None:
         """Synthetic cache contents for decode-only benchmarks (prefill skipped)."""
-        dev = next(t for t in (self.kv, self.k, self.conv_state) if t is not None).device
+        int4 = self.int4 or []
+        dev = next(t for t in (self.kv, self.k, self.conv_state, *(kv.k for kv in int4)) if t is not None).device
         g = torch.Generator(device=dev)
         g.manual_seed(seed)
         for t in (self.kv, self.index_k, self.k, self.v, self.conv_state):
             if t is not None:
                 t.normal_(0.0, std, generator=g)
+        for kv in int4:  # about 3.3 standard deviations each way in 15 steps
+            for codes, scale in ((kv.k, kv.k_scale), (kv.v, kv.v_scale)):
+                codes.random_(0, 256, generator=g)
+                scale[..., 0] = std * 0.44
+                scale[..., 1] = -std * 3.3
         if self.ssm_state is not None:
             self.ssm_state.normal_(0.0, 0.02, generator=g)
 

@@ -68,6 +68,14 @@ def parse_args(argv=None) -> argparse.Namespace:
     ap.add_argument("--enable-expert-parallel", action="store_true")
     ap.add_argument("--enable-prefix-caching", action="store_true",
                     help="reuse the KV blocks of shared prompt prefixes (full-attention models)")
+    ap.add_argument("--kv-cache-dtype", choices=("auto", "int4"), default="auto",
+                    help="int4: grouped-query attention layers cache K and V in 4 bits")
+    ap.add_argument("--kv-cache-budget", type=int, default=None,
+                    help="cached positions a sequence is cut to (needs --kv-cache-dtype int4): the last "
+                         "--kv-cache-recent and the most attended")
+    ap.add_argument("--kv-cache-recent", type=int, default=128)
+    ap.add_argument("--attn-quant", choices=("int8",), default=None,
+                    help="int8: grouped-query attention projections as int8 weights, quantised at load")
     ap.add_argument("--seed", type=int, default=0, help="random-init seed when no checkpoint is given")
     ap.add_argument("--decode-bench", action="store_true",
                     help="take every prompt as prefilled (random cache rows) and only decode: long-ISL decode "
@@ -116,6 +124,10 @@ def main(argv=None) -> None:
         arch = read_hf_config(args.checkpoint)
     else:
         arch = get_preset(args.preset)
+    if args.attn_quant:
+        arch = arch.scaled(attn_quant=args.attn_quant)
+    cache = CacheConfig(enable_prefix_caching=args.enable_prefix_caching, kv_cache_dtype=args.kv_cache_dtype,
+                        kv_budget=args.kv_cache_budget, kv_recent=args.kv_cache_recent)
     dtype = getattr(torch, args.dtype)
     afd = json.loads(args.afd) if args.afd else {}
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -125,7 +137,7 @@ def main(argv=None) -> None:
         ec = EngineConfig(ModelConfig(arch, dtype=dtype, enforce_eager=args.eager, max_model_len=args.max_model_len,
                                       checkpoint=args.checkpoint, seed=args.seed),
                           compilation_config=CompilationConfig(cudagraph_capture_sizes=sizes),
-                          cache_config=CacheConfig(enable_prefix_caching=args.enable_prefix_caching),
+                          cache_config=cache,
                           max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_num_batched_tokens,
                           async_scheduling=args.async_scheduling)
         engine = LLMEngine.colocated(ec, device="cuda" if torch.cuda.is_available() else "cpu")
@@ -175,7 +187,7 @@ def main(argv=None) -> None:
                       parallel_config=ParallelConfig(data_parallel_size=A // args.tp, tensor_parallel_size=args.tp,
                                                      use_ubatching=args.dbo, num_ubatches=2 if args.dbo else 1),
                       compilation_config=CompilationConfig(cudagraph_capture_sizes=sizes),
-                      cache_config=CacheConfig(enable_prefix_caching=args.enable_prefix_caching),
+                      cache_config=cache,
                       additional_config={"afd": dict(afd, role=role)}, max_num_seqs=args.max_num_seqs,
                       max_num_batched_tokens=args.max_num_batched_tokens, async_scheduling=args.async_scheduling)
     if role == "ffn":

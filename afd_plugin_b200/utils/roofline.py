@@ -46,10 +46,10 @@ def weight_bytes_per_step(model) -> int:
     return total
 
 
-def kv_bytes_per_step(arch, context_tokens: int, *, elem_bytes: int = 2) -> int:
+def kv_bytes_per_step(arch, context_tokens: int, *, elem_bytes: float = 2) -> int:
     """Cache bytes read by one decode step over ``context_tokens`` cached positions in total."""
     layers = len(arch.full_attention_layers)
-    return int(context_tokens) * arch.kv_cache_width * elem_bytes * layers
+    return int(int(context_tokens) * arch.kv_cache_width * elem_bytes * layers)
 
 
 __all__ = ["FALLBACK_HBM_GBS", "hbm_peak_gbs", "kv_bytes_per_step", "weight_bytes_per_step"]
