@@ -145,6 +145,9 @@ struct Smem {
   uint32_t tmem_base;
 };
 
+// Of gemm_pair_kernel: 6 stages of 32 KB, channel scales, barriers, padded to 1 KB.
+constexpr size_t kPairSmem = 6 * 2 * kXBytes + 3 * 1024;
+
 struct Args {
   void* y;
   const float* xs;
@@ -426,6 +429,190 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
 }
 
+// Large products: two SMs on one 256 x 256 tile (cta_group::2).  Each CTA of
+// the pair holds half of the tokens (MMA M) and half of the channels (N) in its
+// shared memory; one MMA reads both, so a byte of weights is fetched by one SM
+// for 256 tokens instead of 128, which is what bounds the one-CTA kernel: its
+// tensor pipe is fed 58 B per clock and SM where it could take 94.  CTA 0 issues
+// the MMAs; both CTAs' copies complete on its barriers, and its commits signal
+// both.  Each CTA has its 128 tokens x 256 channels in its own TMEM.
+AFD_DEVICE uint32_t leader_addr(const void* p) {  // the same object in CTA 0 of the cluster
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+AFD_DEVICE void tma_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+AFD_DEVICE void mma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+AFD_DEVICE void commit_pair(uint64_t* bar) {  // arrives on this barrier of both CTAs
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+constexpr int kPairStages = 6;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) gemm_pair_kernel(const __grid_constant__ CUtensorMap x_map,
+                                                                const __grid_constant__ CUtensorMap w_map,
+                                                                const Args a) {
+  constexpr int BN = 256, STAGES = kPairStages;
+  struct SmemT {
+    alignas(1024) uint8_t x[STAGES][kXBytes];
+    alignas(1024) uint8_t w[STAGES][BN / 2 * kBK];
+    alignas(16) float ws[2][BN];
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
+    uint32_t tmem_base;
+  };
+  static_assert(sizeof(SmemT) == kPairSmem, "the launcher's size");
+  extern __shared__ uint8_t smem_raw[];
+  SmemT& sm = *reinterpret_cast<SmemT*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 8);  // the epilogue warps of both CTAs
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                 "r"(2 * BN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  cluster.sync();  // barriers and TMEM of both CTAs are ready
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  const int tiles = a.m_tiles * a.n_tiles, first = blockIdx.x / 2, stride = gridDim.x / 2;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tensormap(&x_map);
+      prefetch_tensormap(&w_map);
+      constexpr uint32_t tx = 2 * (kXBytes + BN / 2 * kBK);  // both CTAs' halves
+      int ahead = 0;  // stages whose weights are on their way before the quantized rows are ready
+      if (first < tiles) {
+        int m, n;
+        tile_at(a, first, m, n);
+        for (; ahead < STAGES && ahead < a.k_blocks; ++ahead) {
+          if (rank == 0) mbar_expect_tx(&sm.full[ahead], tx);
+          tma_pair(sm.w[ahead], &w_map, leader_addr(&sm.full[ahead]), ahead * kBK, n * BN + rank * (BN / 2));
+        }
+      }
+      pdl_wait();
+      int it = 0;
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride) {
+        int m, n;
+        tile_at(a, i, m, n);
+        for (int kb = 0; kb < a.k_blocks; ++kb, ++it) {
+          const int st = it % STAGES;
+          const uint32_t bar = leader_addr(&sm.full[st]);
+          if (it >= ahead) {
+            if (!mbar_wait_bounded(&sm.empty[st], ((it / STAGES) & 1) ^ 1)) {
+              report_timeout(a);
+              ok = false;
+              break;
+            }
+            if (rank == 0) mbar_expect_tx(&sm.full[st], tx);
+            tma_pair(sm.w[st], &w_map, bar, kb * kBK, n * BN + rank * (BN / 2));
+          }
+          tma_pair(sm.x[st], &x_map, bar, kb * kBK, (2 * m + rank) * kBM);
+        }
+      }
+      // no copy of either CTA may still be in flight when they end (at once, unless a wait gave up)
+      if (rank == 0)
+        for (int j = it < STAGES ? 0 : it - STAGES; j < it; ++j)
+          mbar_wait_bounded(&sm.full[j % STAGES], (j / STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc(2 * kBM, BN);
+      int it = 0, acc = 0;
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride, ++acc) {
+        const int ab = acc % 2;
+        if (!mbar_wait_bounded(&sm.acc_empty[ab], ((acc / 2) & 1) ^ 1)) ok = false;
+        tc_fence_after();
+        for (int kb = 0; kb < a.k_blocks && ok; ++kb, ++it) {
+          const int st = it % STAGES;
+          if (!mbar_wait_bounded(&sm.full[st], (it / STAGES) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t xa = smem_u32(sm.x[st]), wa = smem_u32(sm.w[st]);
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            mma_pair(tmem + ab * BN, make_desc(xa + kk * 32), make_desc(wa + kk * 32), idesc, (kb | kk) != 0);
+          commit_pair(&sm.empty[st]);
+        }
+        commit_pair(&sm.acc_full[ab]);
+        if (!ok) {
+          report_timeout(a);
+          mbar_wait_bounded(&sm.acc_full[ab], (acc / 2) & 1);  // no MMA may still write TMEM when it is freed
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
+    pdl_wait();                    // the token scales
+    int acc = 0;
+    for (int i = first; i < tiles; i += stride, ++acc) {
+      const int ab = acc % 2;
+      int m, n;
+      tile_at(a, i, m, n);
+      const int row = (2 * m + rank) * kBM + quarter * 32 + lane;
+      const float xs = row < a.t ? a.xs[row] : 0.f;
+      for (int c = (warp - 2) * 32 + lane; c < BN; c += 128) sm.ws[ab][c] = n * BN + c < a.n ? a.ws[n * BN + c] : 0.f;
+      if (!epi_all(mbar_wait_bounded(&sm.acc_full[ab], (acc / 2) & 1))) {
+        if (lane == 0) report_timeout(a);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t tacc = tmem + ab * BN + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        int v[32];
+        tmem_ld32(tacc + c0, v);
+        store32<T>(a, v, sm.ws[ab] + c0, xs, row, n * BN + c0);
+      }
+      tc_fence_before();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(&sm.acc_empty[ab]))
+                     : "memory");
+    }
+  }
+  tc_fence_before();
+  cluster.sync();  // neither CTA's shared memory or TMEM goes away while the other uses it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+  }
+}
+
 bool encode(CUtensorMap* map, const void* base, int64_t rows, int k, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)k};
@@ -467,6 +654,38 @@ cudaError_t launch(const Int8GemmParams& p, Args a, int splits, cudaStream_t s) 
 }
 
 template <typename T>
+cudaError_t launch_pair(const Int8GemmParams& p, Args a, cudaStream_t s) {
+  a.m_tiles = (p.t + 2 * kBM - 1) / (2 * kBM);
+  a.n_tiles = (p.n + 255) / 256;
+  a.band = (a.band + 1) / 2;
+  a.x_rows = kBM;
+  CUtensorMap xm, wm;
+  if (!encode(&xm, p.xq, p.t, p.k, kBM) || !encode(&wm, p.w, p.n, p.k, 128)) return cudaErrorInvalidValue;
+  auto* kernel = gemm_pair_kernel<T>;
+  const size_t smem = kPairSmem + 1024;
+  static PerDeviceOnce attr;
+  cudaError_t e = attr.run([&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  });
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (int64_t)a.m_tiles * a.n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, device_sm_count() / 2)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, xm, wm, a);
+}
+
+template <typename T>
 cudaError_t run(const Int8GemmParams& p, cudaStream_t s) {
   Args a{};
   a.y = p.y;
@@ -483,6 +702,10 @@ cudaError_t run(const Int8GemmParams& p, cudaStream_t s) {
   a.band = (int)(fit / ((int64_t)kBM * p.k));
   a.band = a.band < 1 ? 1 : (a.band > a.m_tiles ? a.m_tiles : a.band);
   const int sms = device_sm_count();
+  // Enough 256 x 256 tiles for every pair of SMs: 832 us against 928 with one SM
+  // a tile at 4099 x 36864 x 7168, 2.6 POPS (twice the bf16 rate that cuBLAS
+  // sustains there is 2.8).  With at most 128 tokens half a pair would idle.
+  if (a.m_tiles > 1 && (int64_t)((a.m_tiles + 1) / 2) * ((p.n + 255) / 256) >= sms / 2) return launch_pair<T>(p, a, s);
   if ((int64_t)a.m_tiles * ((p.n + 255) / 256) >= sms) return launch<T, 256, 4, false>(p, a, 1, s);
   // Fewer tiles than SMs.  A long contraction is split over a cluster (a share
   // of at least 16 stages: shorter ones cost more to add up than they save); a

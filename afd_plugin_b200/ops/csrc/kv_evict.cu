@@ -8,9 +8,9 @@
 // One cluster of CTAs works on one (sequence, KV head):
 //   1. the CTAs take equal runs of positions and turn scores into 32-bit keys
 //      that order like the scores (in shared memory, as far as they fit);
-//   2. four passes over 8 bits each find the key of the last kept position:
-//      shared-memory histograms, summed over the cluster through distributed
-//      shared memory;
+//   2. four passes over 8 bits each find the key of the last kept position
+//      (the first as the scores arrive): shared-memory histograms, summed over
+//      the cluster through distributed shared memory;
 //   3. each warp counts its run, a prefix over warps and CTAs gives every kept
 //      position its rank;
 //   4. rows move in chunks: all CTAs load a chunk into registers, a cluster
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   constexpr int kRows = kUnits * kEvThreads / kRowUnits;    // rows a CTA moves per chunk
   constexpr int kRowWords = 2 * G + 1;                      // (step, zero) pairs of K and V, and the score
   constexpr int kWords = (kRows * kRowWords + kEvThreads - 1) / kEvThreads;
-  extern __shared__ uint32_t s_keys[];
+  extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ uint32_t s_hist[2][256];
   __shared__ uint32_t s_pick[2];              // digit, positions still to take from it
   __shared__ int s_warp[2][kEvWarps];         // kept-for-sure / tied positions of each warp's run
@@ -92,34 +92,58 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   const EvictView view(p, b, h);
   const int m = n - p.recent;             // candidates
   const int need = p.budget - p.recent;   // of them to keep: 0 <= need < m
-  const int per = (m + cs - 1) / cs;
+  // Runs of whole quads: four positions are one load and one look at the table.
+  const int per = ((m + cs - 1) / cs + 3) & ~3;
   const int lo = min(m, rank * per), cnt = min(m, lo + per) - lo;
+  const int quads = (cnt + 3) / 4;
 
-  auto load_key = [&](int i) { return order_key(p.scores[view.row(lo + i)]); };
-  for (int i = tid; i < min(cnt, p.key_cap); i += kEvThreads) s_keys[i] = load_key(i);
-  auto key_at = [&](int i) { return i < p.key_cap ? s_keys[i] : load_key(i); };
+  uint4* const keys = reinterpret_cast<uint4*>(s_keys);
+  const int held = p.key_cap / 4;  // quads in shared memory; the rest are read again each time
+  auto load_quad = [&](int i) {    // a block's rows come in multiples of 16, so a quad stays inside its block
+    const float4 x = *reinterpret_cast<const float4*>(p.scores + view.row(lo + 4 * i));
+    return make_uint4(order_key(x.x), order_key(x.y), order_key(x.z), order_key(x.w));
+  };
+  auto quad_at = [&](int i) { return i < held ? keys[i] : load_quad(i); };
   for (int i = tid; i < 2 * 256; i += kEvThreads) (&s_hist[0][0])[i] = 0;
   __syncthreads();
 
+  // Adds the digit of one key per lane.  Scores crowd in few exponents: one add
+  // where the warp agrees.  Whole warps call this.
+  auto count_digit = [&](uint32_t* hist, bool in, uint32_t digit) {
+    const uint32_t act = __ballot_sync(0xffffffffu, in);
+    if (act == 0) return;
+    const uint32_t first = __shfl_sync(0xffffffffu, digit, __ffs(act) - 1);
+    if (__all_sync(0xffffffffu, !in || digit == first)) {
+      if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popc(act));
+    } else if (in) {
+      atomicAdd(&hist[digit], 1u);
+    }
+  };
+
   // The key of the last position kept (`bound`) and how many of its ties are.
   uint32_t bound = 0, left = (uint32_t)need;
-  const int padded = (cnt + 31) & ~31;
+  const int padded = (quads + 31) & ~31;
+#pragma unroll 1
   for (int pass = 0; pass < 4; ++pass) {
     const int shift = 24 - 8 * pass;
     uint32_t* hist = s_hist[pass & 1];
+#pragma unroll 2
     for (int i = tid; i < padded; i += kEvThreads) {  // whole warps enter
-      const uint32_t key = i < cnt ? key_at(i) : 0;
-      const bool in = i < cnt && (pass == 0 || (key >> (shift + 8)) == (bound >> (shift + 8)));
-      const uint32_t digit = (key >> shift) & 255u;
-      // Scores crowd in few exponents: one add where a warp agrees.
-      const uint32_t act = __ballot_sync(0xffffffffu, in);
-      if (act == 0) continue;
-      const uint32_t first = __shfl_sync(0xffffffffu, digit, __ffs(act) - 1);
-      if (__all_sync(0xffffffffu, !in || digit == first)) {
-        if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popc(act));
-      } else if (in) {
-        atomicAdd(&hist[digit], 1u);
+      uint4 k4 = make_uint4(0, 0, 0, 0);
+      if (i < quads) {
+        k4 = pass == 0 ? load_quad(i) : quad_at(i);
+        if (pass == 0 && i < held) keys[i] = k4;
       }
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      bool in[4], any = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        in[q] = 4 * i + q < cnt && (pass == 0 || ((k[q] ^ bound) >> (shift + 8)) == 0);
+        any |= in[q];
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) count_digit(hist, in[q], (k[q] >> shift) & 255u);
     }
     cluster.sync();
     uint32_t sum = 0, above = 0;
@@ -156,14 +180,28 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   // left = ties of `bound` to keep, the earliest ones (0 only when need is 0).
   const bool none = need == 0;
 
-  // Each warp's run of positions: its sure and tied counts, then ranks.
-  const int seg = ((cnt + kEvWarps - 1) / kEvWarps + 31) & ~31;
-  const int w0 = min(cnt, warp * seg), w1 = min(cnt, w0 + seg);
+  // Each warp's run of quads: its sure and tied counts (low and high half of one
+  // word), then ranks.
+  const int seg = ((quads + kEvWarps - 1) / kEvWarps + 31) & ~31;
+  const int w0 = min(quads, warp * seg), w1 = min(quads, w0 + seg);
+  auto classes = [&](int i, uint32_t (&c)[4]) {  // 1: above the bound, 1 << 16: tied, 0: out
+    const uint4 k4 = i < w1 ? quad_at(i) : make_uint4(0, 0, 0, 0);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    uint32_t sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool live = !none && i < w1 && 4 * i + q < cnt;
+      c[q] = live && k[q] > bound ? 1u : (live && k[q] == bound ? 1u << 16 : 0u);
+      sum += c[q];
+    }
+    return sum;
+  };
   int gt = 0, eq = 0;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t key = key_at(i);
-    gt += !none && key > bound;
-    eq += !none && key == bound;
+  uint32_t c[4];
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const uint32_t sum = classes(i0 + lane, c);
+    gt += sum & 0xFFFF;
+    eq += sum >> 16;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -192,15 +230,23 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   }
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int i = i0 + lane;
-    const uint32_t key = i < w1 ? key_at(i) : 0;
-    const bool is_gt = i < w1 && !none && key > bound, is_eq = i < w1 && !none && key == bound;
-    const uint32_t mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-    const uint32_t below = (1u << lane) - 1;
-    const int eq_rank = eq_before + __popc(me & below);
-    if (is_gt || (is_eq && eq_rank < (int)left))
-      kept[gt_before + __popc(mg & below) + min(eq_rank, (int)left)] = lo + i;
-    gt_before += __popc(mg);
-    eq_before += __popc(me);
+    const uint32_t mine = classes(i, c);
+    uint32_t upto = mine;  // at most 128 of each in a step: the halves do not meet
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, upto, 31), before = upto - mine;
+    int g = gt_before + (int)(before & 0xFFFF), e = eq_before + (int)(before >> 16);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (c[q] == 1u || (c[q] != 0 && e < (int)left)) kept[g + min(e, (int)left)] = lo + 4 * i + q;
+      g += c[q] & 0xFFFF;
+      e += c[q] >> 16;
+    }
+    gt_before += total & 0xFFFF;
+    eq_before += total >> 16;
   }
   for (int i = rank * kEvThreads + tid; i < p.recent; i += cs * kEvThreads) kept[need + i] = m + i;
   cluster.sync();  // the list is complete, and visible to the cluster
@@ -286,7 +332,7 @@ int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s) {
   // 13.2 and 14.1 us.
   int cs = 1;
   while (cs < 8 && (int64_t)p.batch * p.kv_heads * cs * 2 <= 2 * device_sm_count()) cs *= 2;
-  const int per = (p.max_blocks * p.block_size + cs - 1) / cs;
+  const int per = ((p.max_blocks * p.block_size + cs - 1) / cs + 3) & ~3;
   p.block_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(p.block_size) : -1;
   p.key_cap = per < 46080 ? per : 46080;  // 180 KB
   const size_t smem = (size_t)p.key_cap * 4;

@@ -35,7 +35,9 @@ SHAPES = [  # tokens, n, k
     (1, 1, 16), (3, 7, 48), (8, 32, 128), (5, 5120, 2048), (1, 130, 10944),   # K split over a cluster
     (127, 100, 144), (128, 128, 1024), (129, 257, 528), (256, 2048, 2736),
     (300, 1000, 272), (20, 20000, 256),                                        # one pass of 128-wide tiles
-    (1100, 4500, 400), (2500, 2100, 640), (4099, 1030, 128),                   # 256-wide, several tiles a CTA
+    (1100, 4500, 400), (2500, 2100, 640), (4099, 1030, 128),                   # 256 x 256 on pairs of SMs
+    (129, 19000, 144), (700, 7000, 2048),
+    (100, 40000, 144), (1, 76000, 64),                                         # 128 x 256, several tiles a CTA
 ]
 
 
