@@ -183,3 +183,21 @@ def test_decode_evict_decode():
                     assert all(abs(w[i] - c[i][2]) < 1e-3 for i in range(len(w)))
                     values[b][h] = [c[i] for i in keep]
     assert lens.tolist() == [len(values[b][0]) for b in range(B)]
+
+
+def test_captured_and_replayed():
+    _need_cuda()
+    kv, table, scores = _setup([300, 90, 200], 2, 128, 64, None, "plain", 12)
+    lens = torch.tensor([300, 90, 200], dtype=torch.int32, device="cuda")
+    first = [t.clone() for t in (*kv, scores)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        new, kept = ops.kv_evict_int4(kv, scores, table, lens, 96, 10)
+    for n in ([300, 90, 200], [97, 96, 10]):
+        for t, f in zip((*kv, scores), first):
+            t.copy_(f)
+        lens.copy_(torch.tensor(n))
+        graph.replay()
+        want_kv, want_scores, want_lens, want_kept = _plain(ops.Int4KV(*first[:4]), first[4], table, n, 96, 10)
+        assert new.tolist() == want_lens and torch.equal(kept.cpu(), want_kept)
+        assert all(torch.equal(a, b) for a, b in zip((*kv, scores), (*want_kv, want_scores)))

@@ -337,3 +337,66 @@ def test_two_streams_and_a_replayed_graph():
             gr.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[2])
+
+
+def test_pools_past_32_bit_offsets():
+    """Blocks whose codes lie more than 2^32 bytes into the cache: written, read, attended to and scored."""
+    _need_cuda()
+    g = _gen(21)
+    blocks, bs, hkv, d = 300_000, 64, 4, 128  # 4.9 GB of codes for K and for V
+    kv = ops.int4_kv_cache(blocks, bs, hkv, d)
+    table = torch.tensor([[blocks - 1, 3, 270_001], [280_123, blocks - 2, 0]], dtype=torch.int32, device="cuda")
+    lens = [150, 70]
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    slots = torch.cat([table[b].long()[torch.arange(n, device="cuda") // bs] * bs + torch.arange(n, device="cuda") % bs
+                       for b, n in enumerate(lens)])
+    k, v = (torch.randn(sum(lens), hkv, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    scores = torch.zeros(blocks, hkv, bs, device="cuda")
+    ops.gqa_cache_write_int4(kv, k, v, slots, scores)
+    rk, rv = ops.gqa_cache_read_int4(kv, slots, dtype=torch.float32)
+    assert (rk - k.float()).abs().max() < 0.4 and (rv - v.float()).abs().max() < 0.4  # half a step of about 0.3
+    assert torch.equal(kv.k.view(torch.int32).ne(0).any(-1).any(-1).any(-1).nonzero()[:, 0].cpu(),
+                       torch.tensor([3, 270_001, 280_123, blocks - 2, blocks - 1]))
+    q = torch.randn(2, 32, d, generator=g, device="cuda").bfloat16()
+    out, lse = ops.gqa_decode_int4(q, kv, table, lens_t, 0.1, scores=scores, return_lse=True)
+    _check_decode(q, kv, table, lens, 0.1, out, lse, scores.double())
+    new, kept = ops.kv_evict_int4(kv, scores, table, lens_t, 64, 16)
+    assert new.tolist() == [64, 64] and kept[:, :, -1].tolist() == [[149] * 4, [69] * 4]
+    pos = torch.arange(64, device="cuda")
+    back, _ = ops.gqa_cache_read_int4(kv, table[0].long()[pos // bs] * bs + pos % bs, dtype=torch.float32)
+    for h in range(hkv):
+        assert torch.equal(back[:, h], rk[kept[0, h].long(), h])
+
+
+def test_one_sequence_in_several_rows():
+    """Rows of a batch that share blocks: equal results, and every row's weights in the scores."""
+    _need_cuda()
+    g = _gen(22)
+    kv, table = _pool([600], 2, 128, 64, g)
+    q = torch.randn(1, 8, 128, generator=g, device="cuda").bfloat16().expand(3, -1, -1)
+    lens = torch.full((3,), 600, dtype=torch.int32, device="cuda")
+    one, three = (torch.zeros(kv.k.shape[:3], device="cuda") for _ in range(2))
+    a = ops.gqa_decode_int4(q[:1], kv, table, lens[:1], 0.1, scores=one)
+    b = ops.gqa_decode_int4(q, kv, table.expand(3, -1), lens, 0.1, scores=three)
+    tol = 2.0**-8 * 8 * 1.06 + 1e-3  # another split of the positions: p * step rounded to bf16 at most, steps under 1.06
+    assert all((b[i].float() - a[0].float()).abs().max() <= tol for i in range(3))
+    assert ((three - 3 * one).abs() <= 1e-5 * (1 + three)).all()
+
+
+def test_steps_of_very_different_sizes():
+    """Value steps 2^24 apart inside one head, large keys and queries near the ends of the range."""
+    _need_cuda()
+    g = _gen(23)
+    lens = [900, 40]
+    kv, table = _pool(lens, 1, 128, 64, g)
+    for b, n in enumerate(lens):
+        pos = torch.arange(n, device="cuda")
+        blk, off = table[b].long()[pos // 64], pos % 64
+        for t, spread in ((kv.v_scale, 24), (kv.k_scale, 6)):
+            e = torch.randint(-spread // 2, spread // 2, (n, 1, 2, 1), generator=g, device="cuda")
+            t[blk, :, off] = (t[blk, :, off].float() * torch.exp2(e.float())).bfloat16()
+    for size in (1e-6, 1.0, 1e4):
+        q = (size * torch.randn(2, 8, 128, generator=g, device="cuda")).bfloat16()
+        lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        out, lse = ops.gqa_decode_int4(q, kv, table, lens_t, 0.01 / size, return_lse=True)
+        _check_decode(q, kv, table, lens, 0.01 / size, out, lse)
