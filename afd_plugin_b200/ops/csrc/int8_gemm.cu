@@ -1,8 +1,9 @@
 // Linear layer in 8-bit integers:  y[t, n] = xs[t] ws[n] sum_k xq[t, k] w[n, k].
 //
 // quantize   per token  xs = amax / 127,  xq = clamp(rint(x * (127 / amax)))
-//            with amax = max(|x|, 2^-100); one block per token, the row is
-//            read twice (the second time from cache).
+//            with amax = max(|x|, 2^-100); one block per token, which keeps
+//            a row's first 8192 values in registers (what is longer is read
+//            twice, the second time from cache).
 // gemm       tcgen05.mma kind::i8 on TMA-fed 128B-swizzled tiles, int32
 //            accumulators in TMEM.  int32 sums are exact, so the order and the
 //            split of K do not show in the result; the scales are applied in
@@ -48,35 +49,59 @@ AFD_DEVICE float max_nan(float a, float b) {  // keeps a NaN
   return d;
 }
 
-// 8 consecutive elements as fp32.
+// 8 consecutive elements, as loaded.
 template <typename T>
-AFD_DEVICE void load8(float (&x)[8], const T* p, bool vec) {
-  if (vec) {
-    constexpr int N = Vec16<T>::N;
+struct Chunk {
+  T v[8];
+  AFD_DEVICE void load(const T* p, bool vec) {
+    if (vec) {
+      constexpr int N = Vec16<T>::N;
 #pragma unroll
-    for (int u = 0; u < 8 / N; ++u) {
-      const Vec16<T> v = load16(p + u * N);
+      for (int u = 0; u < 8 / N; ++u) *reinterpret_cast<uint4*>(v + u * N) = *reinterpret_cast<const uint4*>(p + u * N);
+    } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u * N + i] = to_f32(v.v[i]);
+      for (int i = 0; i < 8; ++i) v[i] = p[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
   }
-}
+  AFD_DEVICE float amax(float m) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(to_f32(v[i])));
+    return m;
+  }
+  AFD_DEVICE uint2 quantized(float inv) const {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = max(-127, min(127, __float2int_rn(to_f32(v[i]) * inv)));  // NaN converts to 0; its scale is NaN
+      w[i / 4] |= (uint32_t)(c & 255) << (8 * (i % 4));
+    }
+    return make_uint2(w[0], w[1]);
+  }
+};
+
+constexpr int kQHeld = 4;  // chunks of a row a thread keeps in registers: 8192 values are read once
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) quantize_kernel(int8_t* __restrict__ q, float* __restrict__ scale,
                                                              const T* __restrict__ x, int64_t ld, int k, int vec) {
   __shared__ float s_max[kQThreads / 32];
   pdl_launch_dependents();
+  constexpr int kStride = kQThreads * 8;
   const T* row = x + blockIdx.x * ld;
   int8_t* out = q + (int64_t)blockIdx.x * k;
-  float amax = 0.f, v[8];
-  for (int i = threadIdx.x * 8; i < k; i += kQThreads * 8) {
-    load8(v, row + i, vec != 0);
+  const int i0 = threadIdx.x * 8;
+  Chunk<T> held[kQHeld];
+  float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
+  for (int u = 0; u < kQHeld; ++u)
+    if (i0 + u * kStride < k) held[u].load(row + i0 + u * kStride, vec != 0);
+#pragma unroll
+  for (int u = 0; u < kQHeld; ++u)
+    if (i0 + u * kStride < k) amax = held[u].amax(amax);
+  for (int i = i0 + kQHeld * kStride; i < k; i += kStride) {
+    Chunk<T> c;
+    c.load(row + i, vec != 0);
+    amax = c.amax(amax);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -87,15 +112,13 @@ __global__ void __launch_bounds__(kQThreads) quantize_kernel(int8_t* __restrict_
   for (int w = 0; w < kQThreads / 32; ++w) amax = max_nan(amax, s_max[w]);
   const float inv = __fdiv_rn(127.f, amax);
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(amax, 127.f);
-  for (int i = threadIdx.x * 8; i < k; i += kQThreads * 8) {
-    load8(v, row + i, vec != 0);
-    uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = max(-127, min(127, __float2int_rn(v[j] * inv)));  // NaN converts to 0; its scale is NaN
-      w[j / 4] |= (uint32_t)(c & 255) << (8 * (j % 4));
-    }
-    *reinterpret_cast<uint2*>(out + i) = make_uint2(w[0], w[1]);
+  for (int u = 0; u < kQHeld; ++u)
+    if (i0 + u * kStride < k) *reinterpret_cast<uint2*>(out + i0 + u * kStride) = held[u].quantized(inv);
+  for (int i = i0 + kQHeld * kStride; i < k; i += kStride) {
+    Chunk<T> c;
+    c.load(row + i, vec != 0);
+    *reinterpret_cast<uint2*>(out + i) = c.quantized(inv);
   }
 }
 

@@ -148,7 +148,9 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
     cluster.sync();
     uint32_t sum = 0, above = 0;
     if (tid < 256) {  // thread t looks at digit 255 - t: descending order
-      for (int r = 0; r < cs; ++r) sum += cluster.map_shared_rank(hist, r)[255 - tid];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)  // all loads in flight at once
+        if (r < cs) sum += cluster.map_shared_rank(hist, r)[255 - tid];
       above = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -223,11 +225,13 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
     s_cta[1] = eq_before + eq;
   }
   cluster.sync();
-  for (int r = 0; r < rank; ++r) {
-    const int* other = cluster.map_shared_rank(s_cta, r);
-    gt_before += other[0];
-    eq_before += other[1];
-  }
+#pragma unroll
+  for (int r = 0; r < 7; ++r)
+    if (r < rank) {
+      const int* other = cluster.map_shared_rank(s_cta, r);
+      gt_before += other[0];
+      eq_before += other[1];
+    }
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int i = i0 + lane;
     const uint32_t mine = classes(i, c);
