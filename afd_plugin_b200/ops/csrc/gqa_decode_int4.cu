@@ -11,25 +11,34 @@
 // integers, and the scales stay outside in fp32, as do the running maximum and
 // sum.
 //
-// What bounds it: the packed rows, 144 B per position and KV head at D = 128,
-// at the HBM rate.  A warp unpacks the codes it needs straight into MMA
-// operand registers, so the tile is the A operand (16 positions x 16 dims, or
-// 16 dims x 16 positions) and the query heads are the 8 columns of B: a group
-// of 8 query heads needs half the MMAs that padding the heads to 16 rows
-// would.  Each warp owns whole 16-position tiles: a private ring of cp.async
-// stages, no block barrier in the loop, running maximum and sum per warp; the
-// warps of a CTA merge once at the end.
+// What bounds it: the floor is the packed rows, 144 B per position and KV head
+// at D = 128, at the HBM rate; what it spends is instructions, about 400 a
+// 16-position tile, a third of them the unpacking of codes (the logic pipe is
+// half busy, the tensor pipe a fifth).  16 sequences of 50 - 131 K positions,
+// 32 query heads on 4 KV heads of 128: 835 MB in 212 us, 3.9 TB/s, 60% of the
+// measured copy bandwidth (64% inside the kernel).
+//
+// A warp unpacks the codes it needs straight into MMA operand registers, so
+// the tile is the A operand (16 positions x 16 dims, or 16 dims x 16
+// positions) and the query heads are the 8 columns of B: a group of 8 query
+// heads needs half the MMAs that padding the heads to 16 rows would.  Each
+// warp owns whole tiles: a private ring of cp.async stages, no block barrier
+// in the loop, running maximum and sum per warp; the warps of a CTA merge once
+// at the end, while the next piece's tiles are on their way.
 //
 // Work split: a tile is 16 positions of one (sequence, KV head).  All tiles of
 // the batch, in (sequence, head, position) order, are dealt to one wave of
 // CTAs in equal contiguous shares, whatever the lengths; a share that covers
 // part of a (sequence, head) leaves a partial (unnormalised o, max, sum) that
-// a second small kernel joins.  Short tables (at most kDirectTiles tiles per
-// sequence) take one CTA per (sequence, head) instead and write the result at
-// once: one launch.
+// a second small kernel joins.  Short tables take one CTA per (sequence, head)
+// instead and write the result at once: one launch (kv4_decode_plan).
 //
-// Scores: a second pass over K alone, with the joined log-sum-exp, adds each
-// position's probability (summed over the group's query heads) to its score.
+// Scores: the decode leaves its logits, and a small kernel adds each position's
+// probability under the joined log-sum-exp, summed over the group's query
+// heads, to its score.  Batches whose logits would take more than 512 MB read K
+// once more instead.  Beside the decode alone the two cost 4.3 and 13.9 us at
+// 16 sequences of 0.8 - 2 K positions (16 heads on 16), 13.0 and 17.7 us at 4
+// of 20 - 33 K (64 on 4).
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -80,8 +89,9 @@ AFD_DEVICE constexpr int swz(int row, int chunk) {
 // Tiles a warp takes at once: two where the registers allow it, so that their
 // chains of dependent operations interleave.
 template <int D, int NT> constexpr int kTiles = D * NT <= 128 ? 2 : 1;
-// CTAs one SM holds (their registers bound it).  Measured at 16 sequences of
-// 50 - 131 K positions, D = 128: see the launcher.
+// CTAs one SM holds (their registers bound it).  At 16 sequences of 50 - 131 K
+// positions and D = 128, four CTAs of one tile a step in 128 registers took
+// 239 us, three in 168 registers 220 us.
 template <int D, int NT> constexpr int kResident = D * NT <= 128 ? 3 : 2;
 // Row lengths of query heads and of results in shared memory, padded so that
 // the lanes of one access fall on different banks.
@@ -123,9 +133,8 @@ AFD_DEVICE uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// 2^e of x's binary exponent e + `by`, from the encoding; zero, subnormal and
-// infinite x count as the nearest exponent that keeps the result and its
-// inverse finite.
+// x's binary exponent, from the encoding; zero, subnormal and infinite x count
+// as the nearest one that keeps powers of two near it and their inverses finite.
 AFD_DEVICE int exponent_of(float x) { return min(max((int)(__float_as_uint(x) >> 23) & 255, 40), 214) - 127; }
 AFD_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -294,7 +303,7 @@ struct TileWalk {
       ++pg;
     }
   }
-  // `dst`: this lane's swizzled place in a stage.
+  // `dst`: this lane's swizzled place in a stage (Places::cp).
   template <bool kWithV>
   AFD_DEVICE void load(int u, uint32_t stage, uint32_t dst, int lane) const {
     using R = Ring<D>;
@@ -1115,12 +1124,16 @@ using namespace afd;
 Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len) {
   Kv4Plan plan;
   const int group = heads / kv_heads;
-  // 16 heads share one unpacking of the codes; at D = 256 their accumulators
-  // would not fit in registers, so wider groups take chunks of 8.
+  // 16 heads share one unpacking of the codes: 38.8 us against 41.1 us in two
+  // passes of 8 at 4 sequences of 20 - 33 K positions, 64 heads on 4.  At
+  // D = 256 their accumulators would not fit in registers.
   plan.head_tiles = dim <= 128 && group > 8 ? 2 : 1;
   const int per = 8 * plan.head_tiles;
   plan.chunks = (group + per - 1) / per;
   const int64_t items = (int64_t)batch * kv_heads * plan.chunks;
+  // Up to 512 positions a CTA takes a whole (sequence, head): 6.1 us against
+  // 8.9 us in shares and their join at 2 sequences of up to 61 positions, 10.8
+  // against 15.7 us at 64 of 100 - 512, 27.0 against 35.1 us at 256 of 1 - 512.
   constexpr int kDirectTiles = 32;
   plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
   const int resident = dim * plan.head_tiles <= 128 ? 3 : 2;  // kResident

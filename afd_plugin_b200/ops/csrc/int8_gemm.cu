@@ -18,6 +18,13 @@
 // the quantize kernel: the producer starts on them before it waits for that
 // grid (programmatic dependent launch).
 //
+// What bounds it.  4099 x 36864 x 7168: 700 us in isolation (3.1 POPS), 824 us
+// back to back under the power cap (2.6 POPS; twice cuBLAS's sustained bf16
+// rate is 2.8).  256 x 2048 x 10944: 17.5 us, of which 4 us wait for the
+// quantize kernel and about 6 us feed 90 MB from L2; its floor is 4.4 us of
+// HBM.  5 x 5120 x 2048: 8.3 us, latencies (floor 1.6 us); the call's host work
+// is longer, 11 us.
+//
 // Every wait is bounded; on expiry the CTA records kStatusWaitTimeout, waits
 // (bounded) for its MMAs in flight and winds down.
 #include <cooperative_groups.h>

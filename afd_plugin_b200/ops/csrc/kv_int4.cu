@@ -9,8 +9,10 @@
 //   hold a group, 8 dims each; min and max are three shuffles.
 // read: zero + c * step, one fused multiply-add (the product is exact).
 //
-// Both are bound by memory traffic: one 16-byte load (write) or store (read)
-// per thread and the packed word on the other side.
+// Their floor is memory traffic.  A thread takes K and V of its part of a row,
+// which halves the index arithmetic: 16001 tokens x 8 heads of 128, bf16, are
+// written in 32 us (84 MB, 2.6 TB/s; instruction issue bounds it, 3.3 of 4 per
+// clock) and read as fp32 in 34 us (150 MB, 4.4 TB/s).
 #include "kv_int4.cuh"
 #include "launchers.h"
 
