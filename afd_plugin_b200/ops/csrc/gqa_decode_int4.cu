@@ -1138,7 +1138,9 @@ Kv4Plan kv4_decode_plan(int batch, int heads, int kv_heads, int dim, int max_len
   plan.direct = (max_len + kv4::kTile - 1) / kv4::kTile <= kDirectTiles;
   const int resident = dim * plan.head_tiles <= 128 ? 3 : 2;  // kResident
   plan.ctas = plan.direct ? (int)items : resident * device_sm_count();
-  plan.max_batch = kv4::kMaxBatch;
+  // the prefix sums of a launch stay below 2^31 whatever the lengths
+  const int64_t most = INT32_MAX / ((int64_t)max_len / kv4::kTile + kv4::kRound + kv4::kPieceCost);
+  plan.max_batch = (int)std::min<int64_t>(kv4::kMaxBatch, most);
   return plan;
 }
 
