@@ -503,8 +503,9 @@ float* check_kv4_scores(const c10::optional<at::Tensor>& scores, const at::Tenso
   if (!scores.has_value()) return nullptr;
   check_same_device(*scores, kc, op, "scores");
   TORCH_CHECK(scores->scalar_type() == at::kFloat && scores->is_contiguous() && scores->dim() == 3 &&
-                  scores->size(0) == kc.size(0) && scores->size(1) == kc.size(1) && scores->size(2) == kc.size(2),
-              op, ": fp32 contiguous scores [blocks, kv_heads, block_size]");
+                  scores->size(0) == kc.size(0) && scores->size(1) == kc.size(1) && scores->size(2) == kc.size(2) &&
+                  reinterpret_cast<uintptr_t>(scores->data_ptr()) % 16 == 0,
+              op, ": fp32 contiguous scores [blocks, kv_heads, block_size], 16-byte aligned");
   return scores->data_ptr<float>();
 }
 

@@ -201,3 +201,15 @@ def test_captured_and_replayed():
         want_kv, want_scores, want_lens, want_kept = _plain(ops.Int4KV(*first[:4]), first[4], table, n, 96, 10)
         assert new.tolist() == want_lens and torch.equal(kept.cpu(), want_kept)
         assert all(torch.equal(a, b) for a, b in zip((*kv, scores), (*want_kv, want_scores)))
+
+
+def test_scores_off_a_16_byte_boundary_are_refused():
+    _need_cuda()
+    kv, table, scores = _setup([64], 1, 64, 16, None, "plain", 6)
+    lens = torch.tensor([64], dtype=torch.int32, device="cuda")
+    shifted = torch.zeros(scores.numel() + 1, device="cuda")[1:].view(scores.shape)  # contiguous, 4 bytes off
+    with pytest.raises(RuntimeError, match="16-byte"):
+        ops.kv_evict_int4(kv, shifted, table, lens, 20, 4)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        ops.gqa_decode_int4(torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda"), kv, table, lens, 1.0,
+                            scores=shifted)
