@@ -405,7 +405,8 @@ def kv_evict_int4(
     order, to the sequence's first ``budget`` positions, their scores with them; rows behind those
     stay as they were.  Returns the new lengths, int32 ``[B]``, and the positions kept, ascending,
     int32 ``[B, kv_heads, budget]`` (-1 past a shorter sequence's end).  Sequences of one call must
-    not share blocks: a shared block would be compacted twice.
+    not share blocks: a shared block would be compacted twice.  The budget and the positions that
+    a table row covers are at most 2^30.
     """
     if checks.enabled():
         checks.paged_attention("kv_evict_int4", block_table, seq_lens, num_blocks=kv.num_blocks,
@@ -414,8 +415,10 @@ def kv_evict_int4(
         return _cuda_ops().kv_evict_int4(*kv, scores, block_table, seq_lens, budget, recent)
     kv_int4.check_cache("kv_evict_int4", kv, scores)
     kv_int4.check_batch("kv_evict_int4", block_table, seq_lens, seq_lens.shape[0])
-    if budget < 1 or not 0 <= recent <= budget:
-        raise ValueError(f"kv_evict_int4: 1 <= budget and 0 <= recent <= budget, got {budget} and {recent}")
+    if not 1 <= budget <= 2**30 or not 0 <= recent <= budget:
+        raise ValueError(f"kv_evict_int4: 1 <= budget <= 2^30 and 0 <= recent <= budget, got {budget} and {recent}")
+    if block_table.shape[1] * kv.block_size > 2**30:
+        raise ValueError("kv_evict_int4: a table row covers at most 2^30 positions")
     return ref.kv_evict_int4(kv, scores, block_table, seq_lens, budget, recent)
 
 

@@ -687,8 +687,10 @@ std::tuple<at::Tensor, at::Tensor> kv_evict_int4(at::Tensor& kc, at::Tensor& ks,
   p.scores = check_kv4_scores(scores, kc, op);
   const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
   check_kv4_batch(table, lens, kc, B, op);
-  TORCH_CHECK(budget >= 1 && budget <= INT32_MAX && recent >= 0 && recent <= budget, op,
-              ": 1 <= budget and 0 <= recent <= budget");
+  // the kernel's positions step past the budget and the table by less than 2^30
+  TORCH_CHECK(budget >= 1 && budget <= (1 << 30) && recent >= 0 && recent <= budget, op,
+              ": 1 <= budget <= 2^30 and 0 <= recent <= budget");
+  TORCH_CHECK(table.size(1) * kc.size(2) <= (1 << 30), op, ": a table row covers at most 2^30 positions");
   TORCH_CHECK(B * sh.kv_heads <= (1 << 27), op, ": too many sequences");
   c10::cuda::CUDAGuard g(kc.device());
   auto new_lens = at::empty({B}, lens.options());

@@ -213,3 +213,15 @@ def test_scores_off_a_16_byte_boundary_are_refused():
     with pytest.raises(RuntimeError, match="16-byte"):
         ops.gqa_decode_int4(torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda"), kv, table, lens, 1.0,
                             scores=shifted)
+
+
+def test_positions_past_2_30_are_refused():
+    _need_cuda()
+    kv, table, scores = _setup([64], 1, 64, 16, None, "plain", 7)
+    lens = torch.tensor([64], dtype=torch.int32, device="cuda")
+    wide = torch.zeros(1, 2**26 + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        ops.kv_evict_int4(kv, scores, wide, lens, 4, 1)
+    for budget, recent in ((2**30 + 1, 0), (2**31 - 1, 1)):
+        with pytest.raises(RuntimeError, match="2\\^30"):
+            ops.kv_evict_int4(kv, scores, table, lens, budget, recent)

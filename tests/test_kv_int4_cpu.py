@@ -156,3 +156,14 @@ def test_evict_keeps_the_best_and_the_recent(recent):
     for a in ((0, 0), (4, 5), (4, -1)):
         with pytest.raises(ValueError):
             ops.kv_evict_int4(kv, scores, table, torch.tensor(lens, dtype=torch.int32), *a)
+
+
+def test_evict_refuses_positions_past_2_30():
+    kv = ops.int4_kv_cache(2, 16, 1, 64, device="cpu")
+    scores, lens = torch.zeros(2, 1, 16), torch.zeros(1, dtype=torch.int32)
+    wide = torch.zeros(1, 1, dtype=torch.int32).expand(1, 2**26 + 1)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.kv_evict_int4(kv, scores, wide, lens, 4, 1)
+    for budget, recent in ((2**30 + 1, 0), (2**31, 1)):
+        with pytest.raises(ValueError, match="2\\^30"):
+            ops.kv_evict_int4(kv, scores, wide[:, :2], lens, budget, recent)
