@@ -7,7 +7,7 @@
 //   q . k_t = sum_groups step_t,j * (q_j . c_t,j) + zero_t,j * sum(q_j)
 //   o       = sum_groups (p_t step_t,j) c_t,j + p_t zero_t,j
 // so the tensor cores multiply q (scaled by a power of two per head, exact in
-// fp16) and p * step (rounded to fp16's 11 bits, see take_tile) with small
+// fp16) and p * step (rounded to fp16's 11 bits, see take_tiles) with small
 // integers, and the scales stay outside in fp32, as do the running maximum and
 // sum.
 //
