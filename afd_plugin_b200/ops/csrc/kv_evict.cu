@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   __shared__ int s_warp[2][kEvWarps];         // kept-for-sure / tied positions of each warp's run
   __shared__ int s_cta[2];                    // the CTA's totals, read by the others
   __shared__ uint32_t s_scan[8];
-  __shared__ int64_t s_rows[2][2][kRows];     // source and destination rows of this chunk and the next
+  __shared__ int64_t s_src[2][kRows];         // source rows of this chunk and the next
+  __shared__ int64_t s_dst[3][kRows];         // destination rows, of the last chunk too (see the move)
 
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -260,7 +261,14 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
 
   // Move.  16-byte units of codes and 4-byte words of pairs and scores.  Each
   // row's source and destination are looked up once, by one thread, a chunk
-  // ahead of their use.
+  // ahead of their use.  What orders the lists, with only the cluster barrier
+  // B(i) of chunk i between the threads:
+  //   s_src: chunk i's is written before B(i - 1), read between B(i - 1) and
+  //          B(i), and overwritten (by chunk i + 2's) after B(i): two buffers.
+  //   s_dst: chunk i's is written before B(i - 1) and read by its stores, which
+  //          are between B(i) and B(i + 1), as is the look-up of chunk i + 2.
+  //          That one has a buffer of its own; chunk i + 3's comes after
+  //          B(i + 1): three buffers.
   uint4* const kc = reinterpret_cast<uint4*>(p.k_codes);
   uint4* const vc = reinterpret_cast<uint4*>(p.v_codes);
   auto unit = [&](int64_t row, int u) {
@@ -272,38 +280,41 @@ __global__ void __launch_bounds__(kEvThreads) evict_kernel(Kv4EvictParams p) {
   };
   const int step = cs * kRows, skip = rank * kRows;
   const bool is_dst = tid >= kEvThreads / 2;
-  auto look_up = [&](int buf, int r0) {  // rows r0 .. r0 + kRows - 1
+  auto look_up = [&](int src, int dst, int r0) {  // rows r0 .. r0 + kRows - 1, into these buffers
     for (int r = tid & (kEvThreads / 2 - 1); r < kRows; r += kEvThreads / 2)
-      if (r0 + r < p.budget) s_rows[buf][is_dst][r] = view.row(is_dst ? r0 + r : kept[r0 + r]);
+      if (r0 + r < p.budget) (is_dst ? s_dst[dst] : s_src[src])[r] = view.row(is_dst ? r0 + r : kept[r0 + r]);
   };
-  look_up(0, skip);
+  look_up(0, 0, skip);
   __syncthreads();
-  int buf = 0;
-  for (int r0 = skip; r0 - skip < p.budget; r0 += step, buf ^= 1) {
+  int src = 0, dst = 0;
+  for (int r0 = skip; r0 - skip < p.budget; r0 += step) {
+    const int next_dst = dst == 2 ? 0 : dst + 1;
     uint4 x[kUnits];
     uint32_t y[kWords];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
       const int j = k * kEvThreads + tid, r = j / kRowUnits;
-      if (r0 + r < p.budget) x[k] = *unit(s_rows[buf][0][r], j % kRowUnits);
+      if (r0 + r < p.budget) x[k] = *unit(s_src[src][r], j % kRowUnits);
     }
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int j = k * kEvThreads + tid, r = j / kRowWords;
-      if (j < kRows * kRowWords && r0 + r < p.budget) y[k] = *word(s_rows[buf][0][r], j % kRowWords);
+      if (j < kRows * kRowWords && r0 + r < p.budget) y[k] = *word(s_src[src][r], j % kRowWords);
     }
-    look_up(buf ^ 1, r0 + step);
+    look_up(src ^ 1, next_dst, r0 + step);
     cluster.sync();
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
       const int j = k * kEvThreads + tid, r = j / kRowUnits;
-      if (r0 + r < p.budget) *unit(s_rows[buf][1][r], j % kRowUnits) = x[k];
+      if (r0 + r < p.budget) *unit(s_dst[dst][r], j % kRowUnits) = x[k];
     }
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int j = k * kEvThreads + tid, r = j / kRowWords;
-      if (j < kRows * kRowWords && r0 + r < p.budget) *word(s_rows[buf][1][r], j % kRowWords) = y[k];
+      if (j < kRows * kRowWords && r0 + r < p.budget) *word(s_dst[dst][r], j % kRowWords) = y[k];
     }
+    src ^= 1;
+    dst = next_dst;
   }
 }
 
