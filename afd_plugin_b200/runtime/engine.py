@@ -62,6 +62,7 @@ class Request:
     max_tokens: int
     output: list[int] = field(default_factory=list)
     blocks: list[int] = field(default_factory=list)
+    blocks_epoch: int = 0  # moves on when ``blocks`` changes in another way than by growing
     state_slot: int = -1  # linear-attention state row (Gated DeltaNet models)
     hold_kv: bool = False  # keep the cache rows after finishing, for export to a decode engine
     aborted: bool = False  # ended by abort() before reaching max_tokens
@@ -245,7 +246,7 @@ class LLMEngine:
             t.numpy() for t in (self._h_ids, self._h_pos, self._h_slot, self._h_table, self._h_lens, self._h_next,
                                 self._h_state))
         # (req_id, number of blocks) each staged block-table row holds; rows are rewritten only on change
-        self._row_key: list[tuple[int, int] | None] = [None] * self.max_batch
+        self._row_key: list[tuple[int, int, int] | None] = [None] * self.max_batch
         self.last_h2d_bytes = 0
         self.last_d2h_bytes = 0
         from afd_plugin_b200.utils.profiler import RoleProfiler
@@ -548,6 +549,7 @@ class LLMEngine:
     def _release(self, req: Request) -> None:
         self.kv.allocator.free(req.blocks)
         req.blocks = []
+        req.blocks_epoch += 1  # admitted again, it may have as many blocks, but others
         if req.state_slot >= 0:
             self._free_state_slots.append(req.state_slot)
             req.state_slot = -1
@@ -802,7 +804,7 @@ class LLMEngine:
         self._n_state[:B] = [r.state_slot for r in reqs]
         table, keys = self._n_table, self._row_key
         for i, r in enumerate(reqs):
-            key = (r.req_id, len(r.blocks))
+            key = (r.req_id, r.blocks_epoch, len(r.blocks))
             if keys[i] != key:
                 n = len(r.blocks)
                 table[i, :n] = r.blocks
