@@ -245,7 +245,8 @@ class LLMEngine:
         self._n_ids, self._n_pos, self._n_slot, self._n_table, self._n_lens, self._n_next, self._n_state = (
             t.numpy() for t in (self._h_ids, self._h_pos, self._h_slot, self._h_table, self._h_lens, self._h_next,
                                 self._h_state))
-        # (req_id, number of blocks) each staged block-table row holds; rows are rewritten only on change
+        # (req_id, epoch and number of its blocks) each staged block-table row holds, None for a padding row;
+        # rows are rewritten only on change
         self._row_key: list[tuple[int, int, int] | None] = [None] * self.max_batch
         self.last_h2d_bytes = 0
         self.last_d2h_bytes = 0
@@ -724,8 +725,7 @@ class LLMEngine:
             r.evicted += n - self.kv_budget
             self.kv.allocator.free(r.blocks[keep:])
             del r.blocks[keep:]
-        # a sequence may come back to a block count it had, with other blocks
-        self._row_key = [None] * self.max_batch
+            r.blocks_epoch += 1  # it may come back to a block count it had, with other blocks
         self.num_evictions += len(over)
 
     def _blocks_short(self, r: Request) -> int:

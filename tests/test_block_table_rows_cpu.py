@@ -40,3 +40,36 @@ def test_a_recomputed_request_comes_back_to_its_row_with_other_blocks():
     eng.step()  # recomputed: the same row, as many blocks as before
     assert eng.running[2] is last and len(last.blocks) == len(old) and last.blocks != old
     assert _staged(eng, 3) == _rows(eng, 3)
+
+
+def test_padding_rows_hold_no_blocks_after_a_cut():
+    """One request ends on the step before another is cut to the budget: its row turns into padding."""
+    eng = _engine("tiny-qwen3-moe", block_size=16, kv_cache_dtype="int4", kv_budget=20, kv_recent=4, kv_budget_slack=8)
+    for n, out in ((20, 40), (9, 9)):
+        eng.add_request(list(range(1, n + 1)), out)
+    eng.step()
+    assert _staged(eng, 4) == _rows(eng, 4)
+    while eng.num_evictions == 0:
+        ended = len(eng.running) == 1
+        eng.step()
+    assert ended and len(eng.running) == 1 and len(eng.finished) == 1
+    assert _staged(eng, 4) == _rows(eng, 4)
+
+
+def test_a_cut_request_keeps_its_row():
+    """A cut gives blocks back and the sequence grows again, to a block count it had with other blocks."""
+    eng = _engine("tiny-qwen3-moe", block_size=16, kv_cache_dtype="int4", kv_budget=16, kv_recent=4, kv_budget_slack=20)
+    for n in (20, 30):
+        eng.add_request(list(range(1, n + 1)), 30)
+    eng.step()
+    changed = False
+    seen = {}
+    while eng.running:
+        assert _staged(eng, 3) == _rows(eng, 3)
+        for r in eng.running:
+            old = seen.setdefault((r.req_id, len(r.blocks)), list(r.blocks))
+            changed |= old != r.blocks
+        eng.step()
+        if eng.num_evictions and eng.kv.allocator.num_free > 3:
+            eng.kv.allocator.allocate(1)  # others grow meanwhile
+    assert changed
