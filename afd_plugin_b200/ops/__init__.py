@@ -333,7 +333,7 @@ def gqa_cache_write_int4(
     The slots of one call should differ (rows written to one slot leave a mix of them; padding rows
     share the padding block that way).  A slot outside the cache is skipped and sets the device
     status word.  ``scores`` (the cache's accumulated attention weights) restart at zero there.
-    Values must be finite for their 64-dim group to keep a meaning.
+    A 64-dim group with a NaN, an infinity or a range that overflows fp32 reads back as NaN.
     """
     if checks.enabled():
         checks.cache_slots("gqa_cache_write_int4", slot_mapping, num_slots=kv.num_blocks * kv.block_size)

@@ -63,6 +63,18 @@ template <> AFD_DEVICE float from_f32<float>(float v) { return v; }
 template <> AFD_DEVICE __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> AFD_DEVICE __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// The larger / smaller of two values; a NaN stays one (fmaxf and fminf drop it).
+AFD_DEVICE float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+AFD_DEVICE float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // A 16-byte vector of T (8 x bf16/half or 4 x float).
 template <typename T> struct Vec16 {
   static constexpr int N = 16 / sizeof(T);

@@ -50,12 +50,6 @@ constexpr int kXBytes = kBM * kBK;
 // ------------------------------------------------------------------ quantize
 constexpr int kQThreads = 256;
 
-AFD_DEVICE float max_nan(float a, float b) {  // keeps a NaN
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // 8 consecutive elements, as loaded.
 template <typename T>
 struct Chunk {

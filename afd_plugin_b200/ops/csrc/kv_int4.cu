@@ -5,8 +5,10 @@
 //     c    = clamp(rint(fl(fl(x - zero) / step)), 0, 15)        (0 when step = 0)
 //   zero is rounded down and step up, so every x lies in [zero, zero + 15 step]
 //   and the stored value is within half a step of it.  Every rounding is an
-//   IEEE fp32 operation, so the codes are the same on every device.  8 lanes
-//   hold a group, 8 dims each; min and max are three shuffles.
+//   IEEE fp32 operation, so the codes are the same on every device.  A group
+//   with a NaN, an infinity or a range that overflows fp32 reads back as NaN:
+//   its step is infinite, or step and zero are NaN.  8 lanes hold a group, 8
+//   dims each; min and max are three shuffles.
 // read: zero + c * step, one fused multiply-add (the product is exact).
 //
 // Their floor is memory traffic.  A thread takes K and V of its part of a row,
@@ -71,19 +73,22 @@ AFD_DEVICE void store_group(const float (&x)[8], bool live, uint32_t* word_at, u
   float lo = x[0], hi = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
+    lo = min_nan(lo, x[i]);
+    hi = max_nan(hi, x[i]);
   }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   if (!live) return;
   const float zero = bf16_down(lo);
-  const float step = bf16_up_nonneg(__fdiv_rn(hi - zero, 15.f));
-  uint32_t word = 0;
-  if (step > 1e-25f && step < 1e25f) {
+  const float exact = __fdiv_rn(hi - zero, 15.f);
+  const float step = bf16_up_nonneg(exact);
+  uint32_t word = 0, pair = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
+  if (exact != exact) {  // a NaN in the group, or nothing but one infinity
+    pair = 0x7FC07FC0u;
+  } else if (step > 1e-25f && step < 1e25f) {
     // Adding 1.5 * 2^23 rounds to a whole number, ties to even, in the low bits
     // of 0x4B400000.  zero <= x and the step's rounding keep it in 0 .. 15.
     const float r = __frcp_rn(step);
@@ -98,7 +103,7 @@ AFD_DEVICE void store_group(const float (&x)[8], bool live, uint32_t* word_at, u
       word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - zero, step)), 0.f), 15.f) << (4 * i);
   }
   *word_at = word;
-  if (first) *pair_at = __float_as_uint(step) >> 16 | (__float_as_uint(zero) & 0xFFFF0000u);
+  if (first) *pair_at = pair;
 }
 
 // A block takes kThreads / parts rows (token, head), K and V of each.  D / 8

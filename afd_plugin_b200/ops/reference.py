@@ -124,14 +124,18 @@ def int4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
     ``zero`` is the group's minimum rounded down to bf16, ``step`` is ``(max - zero) / 15`` rounded
     up to bf16, and ``c = clamp(rint((x - zero) / step), 0, 15)``, in fp32 throughout: the stored
-    value ``zero + c * step`` is within half a step of ``x``.
+    value ``zero + c * step`` is within half a step of ``x``.  A group with a NaN, an infinity or a
+    range that overflows fp32 has codes of 0 and reads back as NaN: its step is infinite, or step
+    and zero are NaN.
     """
     g = x.float().unflatten(-1, (-1, INT4_GROUP))
     lo = g.amin(-1, keepdim=True).contiguous()
     bits = lo.view(torch.int32)  # cut to the upper 16 bits; a negative value grows in magnitude first
     zero = (torch.where(bits < 0, bits + 0xFFFF, bits) & -0x10000).view(torch.float32)
     step = (g.amax(-1, keepdim=True) - zero) / g.new_full((1,), 15.0)
-    step = ((step.contiguous().view(torch.int32) + 0xFFFF) & -0x10000).view(torch.float32)
+    bad = step.isnan()
+    zero = torch.where(bad, step, zero)
+    step = torch.where(bad, step, ((step.contiguous().view(torch.int32) + 0xFFFF) & -0x10000).view(torch.float32))
     c = torch.where(step > 0, (g - zero) / step, torch.zeros_like(g)).round().clamp(0, 15)
     c = c.nan_to_num(0.0).to(torch.uint8).flatten(-2)
     return c[..., 0::2] | (c[..., 1::2] << 4), torch.cat([step, zero], -1).bfloat16()
