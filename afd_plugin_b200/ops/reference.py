@@ -134,11 +134,12 @@ def int4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     zero = (torch.where(bits < 0, bits + 0xFFFF, bits) & -0x10000).view(torch.float32)
     step = (g.amax(-1, keepdim=True) - zero) / g.new_full((1,), 15.0)
     bad = step.isnan()
-    zero = torch.where(bad, step, zero)
-    step = torch.where(bad, step, ((step.contiguous().view(torch.int32) + 0xFFFF) & -0x10000).view(torch.float32))
+    zero = torch.where(bad, math.nan, zero)
+    step = torch.where(bad, math.nan, ((step.contiguous().view(torch.int32) + 0xFFFF) & -0x10000).view(torch.float32))
     c = torch.where(step > 0, (g - zero) / step, torch.zeros_like(g)).round().clamp(0, 15)
     c = c.nan_to_num(0.0).to(torch.uint8).flatten(-2)
-    return c[..., 0::2] | (c[..., 1::2] << 4), torch.cat([step, zero], -1).bfloat16()
+    pair = torch.cat([step, zero], -1).contiguous().view(torch.int32) >> 16  # a cast may change a NaN's bits
+    return c[..., 0::2] | (c[..., 1::2] << 4), pair.to(torch.int16).view(torch.bfloat16)
 
 
 def int4_dequantize(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:

@@ -45,3 +45,12 @@ def test_any_nan_payload():
     x[:, 3] = torch.tensor([0x7FFFFFFF, 0x7F800001, -1, -0x7FFFFF], dtype=torch.int32).view(torch.float32)
     codes, scale = ref.int4_quantize(x)
     assert (codes == 0).all() and scale.isnan().all()
+
+
+def test_nan_pairs_have_one_encoding():
+    """The stored pair is the quiet NaN 0x7FC0 in both halves, whatever the vector unit makes of a cast."""
+    for n in (1, 40):  # short and long rows take different paths of a cast
+        x = torch.zeros(n, 64)
+        x[:, 5] = NAN
+        _, scale = ref.int4_quantize(x)
+        assert (scale.view(torch.int16) == 0x7FC0).all()
