@@ -371,7 +371,8 @@ def gqa_decode_int4(
     """Single-token attention ``[B, heads, d]`` of ``q [B, heads, d]`` (bf16 / fp16) over the 4-bit cache.
 
     An empty sequence gives zeros (and a log-sum-exp of ``-inf``).  With ``return_lse`` also the
-    natural log-sum-exp of every row, fp32 ``[B, heads]``.  With ``scores``
+    natural log-sum-exp of every row, fp32 ``[B, heads]``.  Stored keys and values are taken up to
+    2^100 in magnitude.  With ``scores``
     (``[blocks, kv_heads, block_size]`` fp32) each cached position's attention weight, summed over
     the query heads that share its KV head, is added to its entry: the weight :func:`kv_evict_int4`
     keeps positions by.  Sequences of a batch that share blocks add to the same entries, in no fixed

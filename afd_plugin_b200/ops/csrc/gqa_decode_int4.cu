@@ -58,6 +58,7 @@ constexpr int kDecThreads = kWarps * 32;
 constexpr int kMaxBatch = 256;       // sequences per launch (their prefix sums sit in shared memory)
 constexpr float kLowest = -FLT_MAX;  // a maximum before any logit: finite, so that differences stay defined
 constexpr float kStepTop = 512.f;    // scaled steps stay below this (times 2^kLazy: fp16 factors below 2^15)
+constexpr int kScaleTop = 117;       // steps of 2^-108 and more set their own scale, smaller ones keep 2^117
 constexpr float kLazy = 6.f;         // the running maximum moves when it is exceeded by 2^6
 // What a piece costs beside its tiles (pipeline fill, query, merge), in tiles,
 // and the steps of all warps that tiles come in.  Measured at 256 sequences of
@@ -133,9 +134,9 @@ AFD_DEVICE uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// x's binary exponent, from the encoding; zero, subnormal and infinite x count
-// as the nearest one that keeps powers of two near it and their inverses finite.
-AFD_DEVICE int exponent_of(float x) { return min(max((int)(__float_as_uint(x) >> 23) & 255, 40), 214) - 127; }
+// x's binary exponent, from the encoding, as -112 .. 127: 2^(5 - it), 2^(14 - it)
+// and their inverses are normal numbers, for subnormal and infinite x too.
+AFD_DEVICE int exponent_of(float x) { return min(max((int)(__float_as_uint(x) >> 23) & 255, 15), 254) - 127; }
 AFD_DEVICE float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // 8x8 transpose of 16-bit values held one row pair per lane.
@@ -520,7 +521,7 @@ struct Acc {
       l[t][0] = l[t][1] = 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < G; ++j) scale[j] = pow2(87);
+    for (int j = 0; j < G; ++j) scale[j] = pow2(kScaleTop);
   }
 };
 
