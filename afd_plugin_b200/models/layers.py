@@ -337,8 +337,9 @@ def _attend_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: Attent
         pos = torch.arange(int(meta.positions[start:end].max()) + 1, device=q.device)
         slots = meta.block_table[seq].long()[pos // bs] * bs + pos % bs
         ks, vs = ops.gqa_cache_read_int4(cache.kv, slots, dtype=q.dtype)
-        o[start:end], weights = ref.gqa_attend(q[start:end], ks, vs, meta.positions[start:end], scale)
-        if cache.scores is not None:
+        o[start:end], weights = ref.gqa_attend(q[start:end], ks, vs, meta.positions[start:end], scale,
+                                               with_weights=cache.scores is not None)
+        if weights is not None:
             heads = torch.arange(weights.shape[0], device=q.device)[:, None]
             cache.scores.index_put_((slots // bs, heads, slots % bs), weights, accumulate=True)
     return o

@@ -528,11 +528,11 @@ def gqa_prefill(
                       scale)[0]
 
 
-def gqa_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
-               scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+def gqa_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, scale: float,
+               with_weights: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Causal attention of queries at ``positions`` over the rows ``k`` / ``v [n, kv_heads, d]`` of
-    positions ``0 .. n - 1``: the output, and each row's attention weight summed over the queries
-    and the query heads that share its KV head (``[kv_heads, n]`` fp32)."""
+    positions ``0 .. n - 1``: the output, and ``with_weights`` each row's attention weight summed over
+    the queries and the query heads that share its KV head (``[kv_heads, n]`` fp32)."""
     T, Hq, D = q.shape
     n, Hkv = k.shape[:2]
     qf = q.float().view(T, Hkv, Hq // Hkv, D)
@@ -540,7 +540,8 @@ def gqa_attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     mask = torch.arange(n, device=q.device)[None, :] > positions.long()[:, None]
     s = s.masked_fill(mask[:, None, None, :], float("-inf"))
     p = torch.softmax(s, dim=-1)
-    return torch.einsum("tkgn,nkd->tkgd", p, v.float()).reshape(T, Hq, D).to(q.dtype), p.sum((0, 2))
+    o = torch.einsum("tkgn,nkd->tkgd", p, v.float()).reshape(T, Hq, D).to(q.dtype)
+    return o, p.sum((0, 2)) if with_weights else None
 
 
 # ------------------------------------------------------ gated delta net (linear attention)
