@@ -348,7 +348,10 @@ def gqa_cache_write_int4(
 def gqa_cache_read_int4(
     kv: Int4KV, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    """The values stored at ``slots [n]`` (int64): ``(k, v)``, each ``[n, kv_heads, d]`` in ``dtype``."""
+    """The values stored at ``slots [n]`` (int64): ``(k, v)``, each ``[n, kv_heads, d]`` in ``dtype``.
+
+    A slot outside the cache reads as zeros and sets the device status word.
+    """
     if checks.enabled():
         checks.cache_slots("gqa_cache_read_int4", slots, num_slots=kv.num_blocks * kv.block_size)
     if _cuda(slots):

@@ -152,7 +152,11 @@ def int4_dequantize(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 def gqa_cache_write_int4(kv, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
                          scores: torch.Tensor | None = None) -> None:
     bs = kv.k.shape[2]
-    blk, off = slot_mapping.long() // bs, slot_mapping.long() % bs
+    slots = slot_mapping.long()
+    inside = (slots >= 0) & (slots < kv.k.shape[0] * bs)
+    if not inside.all():  # skipped
+        slots, k, v = slots[inside], k[inside], v[inside]
+    blk, off = slots // bs, slots % bs
     kv.k[blk, :, off], kv.k_scale[blk, :, off] = int4_quantize(k)
     kv.v[blk, :, off], kv.v_scale[blk, :, off] = int4_quantize(v)
     if scores is not None:
@@ -161,9 +165,15 @@ def gqa_cache_write_int4(kv, k: torch.Tensor, v: torch.Tensor, slot_mapping: tor
 
 def gqa_cache_read_int4(kv, slots: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     bs = kv.k.shape[2]
-    blk, off = slots.long() // bs, slots.long() % bs
-    return (int4_dequantize(kv.k[blk, :, off], kv.k_scale[blk, :, off]).to(dtype),
-            int4_dequantize(kv.v[blk, :, off], kv.v_scale[blk, :, off]).to(dtype))
+    inside = (slots >= 0) & (slots < kv.k.shape[0] * bs)
+    at = torch.where(inside, slots.long(), 0)
+    blk, off = at // bs, at % bs
+
+    def one(codes, scale):
+        x = int4_dequantize(codes[blk, :, off], scale[blk, :, off])
+        return torch.where(inside[:, None, None], x, 0.0).to(dtype)  # zeros outside the cache
+
+    return one(kv.k, kv.k_scale), one(kv.v, kv.v_scale)
 
 
 def _int4_positions(block_row: torch.Tensor, n: int, block_size: int) -> torch.Tensor:
