@@ -415,6 +415,7 @@ def kv_evict_int4(
     if checks.enabled():
         checks.paged_attention("kv_evict_int4", block_table, seq_lens, num_blocks=kv.num_blocks,
                                block_size=kv.block_size, min_len=0)
+        checks.unshared_blocks("kv_evict_int4", block_table, seq_lens, block_size=kv.block_size, rewritten=budget)
     if _cuda(scores):
         return _cuda_ops().kv_evict_int4(*kv, scores, block_table, seq_lens, budget, recent)
     kv_int4.check_cache("kv_evict_int4", kv, scores)

@@ -65,6 +65,22 @@ def paged_attention(op: str, block_table: torch.Tensor, seq_lens: torch.Tensor, 
                                f"[0, {num_blocks})")
 
 
+def unshared_blocks(op: str, block_table: torch.Tensor, seq_lens: torch.Tensor, *, block_size: int,
+                    rewritten: int) -> None:
+    """No block of a sequence longer than ``rewritten`` positions, whose rows the call moves, appears twice."""
+    if not _active(block_table):
+        return
+    bt = block_table.detach().to("cpu", torch.int64)
+    sl = seq_lens.detach().to("cpu", torch.int64).view(-1)
+    used = (torch.arange(bt.shape[1])[None, :] < ((sl + block_size - 1) // block_size)[:, None]).nonzero()
+    owner: dict[int, tuple[int, int]] = {}
+    for b, i in used.tolist():
+        other = owner.setdefault(int(bt[b, i]), (b, i))
+        if other != (b, i) and max(int(sl[b]), int(sl[other[0]])) > rewritten:
+            raise KernelInputError(f"{op}: block_table[{b}, {i}] = {int(bt[b, i])} is block_table[{other[0]}, "
+                                   f"{other[1]}] too: a moved block must not be shared")
+
+
 def cache_slots(op: str, slot_mapping: torch.Tensor, *, num_slots: int) -> None:
     if not _active(slot_mapping):
         return
@@ -101,4 +117,4 @@ def expert_ids(op: str, ids: torch.Tensor, *, num_experts: int | None = None,
 
 
 __all__ = ["ENV", "KernelInputError", "cache_slots", "enable", "enabled", "expert_ids", "paged_attention",
-           "state_slots"]
+           "state_slots", "unshared_blocks"]
