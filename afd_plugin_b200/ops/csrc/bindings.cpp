@@ -461,8 +461,8 @@ int* status_ptr_or_null(const at::Tensor& like) {
   return status_ptr(like);
 }
 
-// Numbers in messages go through std::to_string: the extension may carry its own
-// copy of the C++ runtime, whose stream formatting of numbers is not usable here.
+// Numbers in messages go through std::to_string: a build that carries its own copy
+// of the C++ runtime could not format them in a stream (see setup.py).
 struct Kv4Shape {
   int blocks, kv_heads, block_size, dim;
 };

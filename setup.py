@@ -4,6 +4,7 @@ Produces ``afd_plugin_b200/_C*.so`` (loaded with ``torch.ops.load_library``).
 Kernels are compiled for sm_100a only (tcgen05 / TMA code paths).
 """
 
+import ctypes.util
 import glob
 import os
 
@@ -26,6 +27,9 @@ def _nccl_dirs():
 
 
 NCCL_INC, NCCL_LIB = _nccl_dirs()
+# The C++ runtime that PyTorch has loaded, by soname: some toolchains link a static copy of their own,
+# whose locale is never set up, and formatting a number into an error message then ends the process.
+STDCXX = ["-l:libstdc++.so.6"] if ctypes.util.find_library("stdc++") == "libstdc++.so.6" else []
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 DEBUG = os.environ.get("AFD_B200_KERNEL_DEBUG", "") in ("1", "true", "on")
 
@@ -48,7 +52,8 @@ setup(
             include_dirs=[os.path.join(ROOT, CSRC)] + NCCL_INC,
             library_dirs=NCCL_LIB,
             # libnccl.so.2 is the library PyTorch itself loads (resolved by soname at load time)
-            extra_link_args=[f"-Wl,-rpath,{d}" for d in NCCL_LIB] + (["-l:libnccl.so.2"] if NCCL_LIB else ["-lnccl"]),
+            extra_link_args=[f"-Wl,-rpath,{d}" for d in NCCL_LIB] + (["-l:libnccl.so.2"] if NCCL_LIB else ["-lnccl"])
+            + STDCXX,
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": nvcc_flags},
         )
     ],
