@@ -7,9 +7,9 @@
 //   q . k_t = sum_groups step_t,j * (q_j . c_t,j) + zero_t,j * sum(q_j)
 //   o       = sum_groups (p_t step_t,j) c_t,j + p_t zero_t,j
 // so the tensor cores multiply q (scaled by a power of two per head, exact in
-// fp16) and p * step (rounded to fp16's 11 bits, see take_tiles) with small
-// integers, and the scales stay outside in fp32, as do the running maximum and
-// sum.
+// fp16) and p * step (rounded to fp16's 11 bits, or 22 for fp16 results, see
+// take_tiles) with small integers, and the scales stay outside in fp32, as do
+// the running maximum and sum.
 //
 // What bounds it: the floor is the packed rows, 144 B per position and KV head
 // at D = 128, at the HBM rate; what it spends is instructions, about 400 a
@@ -529,7 +529,12 @@ struct Acc {
 // first tile on exist (kTail: fewer than the step's): the others weigh nothing,
 // whatever their bytes hold.
 //
-// The second product takes p * step in fp16, 11 bits.  p is at most 2^kLazy,
+// The second product takes p * step in fp16, 11 bits: half a step of that is an
+// eighth of the half step of a bf16 result.  An fp16 result, whose half step it
+// would equal, takes what the first factor leaves as a second one (22 bits): at
+// 16 sequences of 50 - 131 K positions 239 us instead of 217, at 16 of 0.8 - 2 K
+// with scores 34.5 instead of 32.7; the error against 64 bits is 1.9 - 2.1e-4,
+// the result's own rounding, instead of 2.6e-4.  p is at most 2^kLazy,
 // and a power of two per dim group (kept per warp, lowered when a larger step
 // comes) holds the steps below 2^9, so the factors stay below 2^15.  A step
 // that set the scale gets 2^5 at least: factors keep full precision down to
@@ -540,6 +545,7 @@ AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t s
                            int heads) {
   using R = Ring<D>;
   constexpr int G = D / kGroup, U = kTiles<D, NT>;
+  constexpr int kParts = std::is_same<T, __half>::value ? 2 : 1;
   float s[U][NT][4];
 #pragma unroll
   for (int u = 0; u < U; ++u) tile_logits<T, D, NT>(s[u], q, stage + u * R::kStageBytes, at, codes, shl16);
@@ -653,14 +659,22 @@ AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t s
     for (int j = 0; j < G; ++j) {
       const float z0 = fmaf(8.f, st[u][0][j], pair_zero(pr[u][0][j]));
       const float z1 = fmaf(8.f, st[u][1][j], pair_zero(pr[u][1][j]));
-      uint32_t b[NT][2];
+      uint32_t b[NT][kParts][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float* p = s[u][t];
         acc.zo[t][j][0] = fmaf(p[0], z0, fmaf(p[2], z1, acc.zo[t][j][0]));
         acc.zo[t][j][1] = fmaf(p[1], z0, fmaf(p[3], z1, acc.zo[t][j][1]));
-        b[t][0] = transpose8(pack_f16(p[0] * k[u][0][j], p[1] * k[u][0][j]));
-        b[t][1] = transpose8(pack_f16(p[2] * k[u][1][j], p[3] * k[u][1][j]));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float lo = p[2 * r] * k[u][r][j], hi = p[2 * r + 1] * k[u][r][j];
+          const uint32_t top = pack_f16(lo, hi);
+          b[t][0][r] = transpose8(top);
+          if constexpr (kParts == 2) {
+            const float2 took = __half22float2(*reinterpret_cast<const __half2*>(&top));
+            b[t][1][r] = transpose8(pack_f16(lo - took.x, hi - took.y));
+          }
+        }
       }
       // k indices 2c, 2c + 1, 2c + 8, 2c + 9 are rows c, c + 4, c + 8, c + 12
       const uint32_t even = ((stage + at.v) ^ (j * 32)) + u * R::kStageBytes;
@@ -675,7 +689,10 @@ AFD_DEVICE void take_tiles(Acc<D, NT>& acc, const Query<T, D, NT>& q, uint32_t s
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_f16(acc.o[t][j * 4 + i], x0[i], x1[i], x2[i], x3[i], b[t][0], b[t][1]);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+            mma_f16(acc.o[t][j * 4 + i], x0[i], x1[i], x2[i], x3[i], b[t][part][0], b[t][part][1]);
     }
   }
 }
