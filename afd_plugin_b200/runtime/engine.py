@@ -192,8 +192,12 @@ class LLMEngine:
         self._free_state_slots = list(range(self.max_batch - 1, -1, -1))
         self.ffn = ffn_executor or LocalFFNExecutor(model)
         num_ub = engine_config.parallel_config.num_ubatches if engine_config.parallel_config.use_ubatching else 1
+        # a decode step follows a cut: its sequences hold budget + slack positions at most, the new one among them
+        decode_blocks = (None if cc.kv_budget is None
+                         else math.ceil((cc.kv_budget + cc.kv_budget_slack) / self.block_size))
         self.runner = ModelRunner(model, self.kv, self.ffn, max_batch=self.max_batch,
-                                  max_blocks_per_seq=self.max_blocks_per_seq, num_ubatches=num_ub)
+                                  max_blocks_per_seq=self.max_blocks_per_seq, num_ubatches=num_ub,
+                                  decode_blocks=decode_blocks)
         self.coordinator = coordinator or AttentionCoordinator()
         # Prefix caching shares KV blocks between prompts; recurrent (Gated
         # DeltaNet) state is per request, so hybrid models never share.

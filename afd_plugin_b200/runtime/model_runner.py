@@ -81,13 +81,17 @@ class ModelRunner:
         max_batch: int,
         max_blocks_per_seq: int,
         num_ubatches: int = 1,
+        decode_blocks: int | None = None,
     ):
+        """``decode_blocks``: the most blocks a decoded sequence has (default: ``max_blocks_per_seq``); attention
+        sizes its workspaces by the block table it is given."""
         self.model = model
         self.kv = kv_cache
         self.ffn = ffn_executor
         self.device = model.device
         self.max_batch = max_batch
         self.max_blocks = max_blocks_per_seq
+        self.decode_blocks = max_blocks_per_seq if decode_blocks is None else min(decode_blocks, max_blocks_per_seq)
         self.num_ubatches = num_ubatches
         self.buf = DecodeBuffers.allocate(max_batch, max_blocks_per_seq, self.device)
         self.graphs: dict[int, _Graph] = {}
@@ -157,7 +161,7 @@ class ModelRunner:
             metas.append(AttentionMetadata(
                 positions=b.positions[lo:hi],
                 slot_mapping=b.slot_mapping[lo:hi],
-                block_table=b.block_table[lo:hi],
+                block_table=b.block_table[lo:hi, : self.decode_blocks],
                 seq_lens=b.seq_lens[lo:hi],
                 is_decode=True,
                 state_slots=b.state_slots[lo:hi] if self.has_linear_state else None,
