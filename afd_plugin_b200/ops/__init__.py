@@ -378,8 +378,9 @@ def gqa_decode_int4(
     2^100 in magnitude.  With ``scores``
     (``[blocks, kv_heads, block_size]`` fp32) each cached position's attention weight, summed over
     the query heads that share its KV head, is added to its entry: the weight :func:`kv_evict_int4`
-    keeps positions by.  Sequences of a batch that share blocks add to the same entries, in no fixed
-    order.
+    keeps positions by.  Adds to one entry have no fixed order where sequences of a batch share blocks,
+    and where a KV head has more than 16 query heads (8 at dim 256) and a launch's logits would take
+    more than 512 MB (the table's width counts): such scores may differ in their last bits.
     """
     if checks.enabled():
         checks.paged_attention("gqa_decode_int4", block_table, seq_lens, num_blocks=kv.num_blocks,

@@ -12,10 +12,11 @@
 // the running maximum and sum.
 //
 // What bounds it: the floor is the packed rows, 144 B per position and KV head
-// at D = 128, at the HBM rate; what it spends is instructions, about 400 a
-// 16-position tile, a third of them the unpacking of codes (the logic pipe is
-// half busy, the tensor pipe a fifth).  16 sequences of 50 - 131 K positions,
-// 32 query heads on 4 KV heads of 128: 835 MB in 212 us, 3.9 TB/s, 60% of the
+// at D = 128, at the HBM rate; what it spends is the latency of about 400
+// instructions a 16-position tile, a third of them the unpacking of codes, at
+// 12 warps per SM (2.4 instructions a clock of 4; the logic pipe is half busy,
+// the tensor pipe a fifth).  16 sequences of 50 - 131 K positions, 32 query
+// heads on 4 KV heads of 128, bf16: 835 MB in 215 us, 3.9 TB/s, 59% of the
 // measured copy bandwidth (64% inside the kernel).
 //
 // A warp unpacks the codes it needs straight into MMA operand registers, so

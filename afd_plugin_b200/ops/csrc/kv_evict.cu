@@ -346,8 +346,9 @@ using namespace afd;
 int launch_kv_evict_int4(Kv4EvictParams p, int dim, cudaStream_t s) {
   // As many CTAs on each (sequence, head) as keep all of them resident at once,
   // two per SM.  Measured at 128 (sequences x heads) of 20 - 33 K positions:
-  // 170, 123, 133 and 159 us with 1, 2, 4 and 8; at 12 of 1.1 K: 20.7, 15.7,
-  // 13.2 and 14.1 us.
+  // 170, 123, 133 and 159 us with 1, 2, 4 and 8, where the rule takes 2; at 12
+  // of 1.1 K 20.7, 15.7, 13.2 and 14.1 us, where it takes 8, a microsecond from
+  // the best.
   int cs = 1;
   while (cs < 8 && (int64_t)p.batch * p.kv_heads * cs * 2 <= 2 * device_sm_count()) cs *= 2;
   const int per = ((p.max_blocks * p.block_size + cs - 1) / cs + 3) & ~3;
