@@ -194,6 +194,8 @@ class ModelRunner:
         Used by device-resident decode loops (benchmarks); rows must own KV
         blocks for the next position already.
         """
+        if self.decode_blocks < self.max_blocks:
+            raise ValueError("a device-resident decode loop does not cut its sequences to the cache budget")
         from afd_plugin_b200.ops._ext import ops as cuda_ops
 
         b = self.buf

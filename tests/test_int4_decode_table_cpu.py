@@ -45,3 +45,10 @@ def test_tables_without_a_budget_or_with_a_large_one(seen):
     _engine().generate([[1, 2, 3]], 3)
     _engine(kv_budget=150, kv_recent=8, kv_budget_slack=100).generate([[1, 2, 3]], 3)
     assert {w for w, _ in seen} == {10}
+
+
+def test_device_resident_loops_refuse_a_budget():
+    """They move every row on without a cut, past what the bounded table holds."""
+    eng = _engine(kv_budget=32, kv_recent=8)
+    with pytest.raises(ValueError, match="cache budget"):
+        eng.runner.advance_on_device(1)
